@@ -1,0 +1,243 @@
+// Decode attention of one new token over selected pages.
+//
+// For a row and a kv head the caller lists pages of the row's sequence (hkb_select_pages); the group's query heads
+// attend to the tokens of those pages that lie below the sequence's length:
+//   out = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale k_scale q.k_t - max),  lse = max + log sum_t p_t.
+//
+// Bound: bytes (the selected K and V rows once, 4 to 16 flop a byte). A cluster of `splits` CTAs takes a (row, kv
+// head); the 16-token tiles of its pages are dealt to all the cluster's warps in turn, each warp a cp.async ring and
+// an online softmax of its own (the decode walk's workers, fragments and all). The warps' normalised partials stay
+// in shared memory, and after one cluster barrier every CTA folds its slice of the outputs out of its peers' memory:
+// one launch, no scratch, nothing shared between calls.
+#include "hkb_cluster.cuh"
+#include "hkb_walk_mma.cuh"
+
+namespace hkb {
+
+struct SparseArgs {
+  DecodeArgs d;                  // q, caches, table, lengths, scales; the split scratch is not used
+  const int* pages;              // (row, kv head): `budget` pages of the sequence, a negative entry is none
+  int64_t p_stride_row, p_stride_head;
+  int budget;
+  float* out_lse;                // (rows, q heads) or null
+};
+
+template <class P, int WARPS, bool F16>
+__global__ void __launch_bounds__(WARPS * 32) sparse_kernel(const SparseArgs a) {
+  extern __shared__ __align__(128) uint8_t hkb_smem[];
+  constexpr int D = P::HEAD_DIM, HEADS = P::HEADS, NST = P::STAGES;
+  static_assert(HEADS * (D + 1) * 4 <= P::RING_SMEM, "a warp's partial lies where its ring was");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int ctas = cluster_size(), rank = cluster_rank();
+  const int kvh = blockIdx.y, row = blockIdx.z;
+  const int nh = a.d.group, hq0 = kvh * nh;
+  const int seq_len = max(__ldg(a.d.seq_lens + row), 0);
+
+  float qs = a.d.scale * LOG2E, vs = 1.f;
+  if (a.d.k_scale) qs *= __ldg(a.d.k_scale);
+  if (a.d.v_scale) vs = __ldg(a.d.v_scale);
+
+  typename P::Loader ld;
+  ld.kbase = a.d.k + (int64_t)kvh * a.d.k_stride_head;
+  ld.vbase = a.d.v + (int64_t)kvh * a.d.v_stride_head;
+  ld.ksb = a.d.k_stride_block; ld.kst = a.d.k_stride_token;
+  ld.vsb = a.d.v_stride_block; ld.vst = a.d.v_stride_token;
+  ld.tiles_per_page = a.d.tiles_per_page; ld.num_blocks = a.d.num_blocks;
+  ld.prepare(lane);
+
+  // The warp's tiles: every `workers`-th of the list's budget x tiles_per_page, 32 looked up at a time, a batch ahead.
+  const int* list = a.pages + (int64_t)row * a.p_stride_row + (int64_t)kvh * a.p_stride_head;
+  const int* table = a.d.block_table + (int64_t)row * a.d.table_stride;
+  const int workers = ctas * WARPS, tpp = a.d.tiles_per_page, total = a.budget * tpp;
+  auto look_up = [&](int i0, int& id, int& tok) {     // lane l: item i0 + l; tok < 0: no tile
+    id = 0; tok = -1;
+    const int64_t x = (int64_t)(i0 + lane) * workers + rank * WARPS + warp;
+    if (x >= total) return;
+    const int e = (int)x / tpp, sub = (int)x - e * tpp;
+    const int p = __ldg(list + e);
+    if (p < 0 || p >= a.d.max_pages) return;
+    const int64_t t0 = (int64_t)p * a.d.block_size + sub * TILE_TOKENS;
+    if (t0 >= seq_len) return;
+    tok = (int)t0;
+    id = __ldg(table + p);
+  };
+  int next_item = 64, id, tok, id_n, tok_n;
+  look_up(0, id, tok);
+  look_up(32, id_n, tok_n);
+  unsigned live = __ballot_sync(0xffffffffu, tok >= 0);
+  const uint32_t ring = smem_u32(hkb_smem) + warp * P::RING_SMEM;
+  // Requests the warp's next tile into a ring stage; its first token, or -1 where none is left.
+  auto issue = [&](int stage) -> int {
+    while (!live) {
+      if ((int64_t)(next_item - 32) * workers >= total) return -1;
+      id = id_n; tok = tok_n;
+      live = __ballot_sync(0xffffffffu, tok >= 0);
+      look_up(next_item, id_n, tok_n);
+      next_item += 32;
+    }
+    const int src = __ffs(live) - 1;
+    live &= live - 1;
+    const int t = __shfl_sync(0xffffffffu, tok, src);
+    ld.issue(ring + stage * P::STAGE_BYTES, t / TILE_TOKENS, __shfl_sync(0xffffffffu, id, src), lane);
+    return t;
+  };
+  int queue[NST - 1];            // first tokens of the tiles in flight, oldest first
+#pragma unroll
+  for (int k = 0; k < NST - 1; ++k) { queue[k] = issue(k); cp_async_commit(); }
+
+  typename P::State st;
+  P::begin(st, a.d, row, hq0, nh, lane, qs);
+  int sc = 0, sl = NST - 1;
+  while (queue[0] >= 0) {
+    cp_async_wait<NST - 2>();
+    __syncwarp();
+    const int t = issue(sl);
+    cp_async_commit();
+    P::step(st, ring, sc, queue[0], seq_len, queue[0] + TILE_TOKENS > seq_len, lane, qs);
+#pragma unroll
+    for (int k = 0; k + 1 < NST - 1; ++k) queue[k] = queue[k + 1];
+    queue[NST - 2] = t;
+    sc = sc + 1 == NST ? 0 : sc + 1;
+    sl = sl + 1 == NST ? 0 : sl + 1;
+  }
+  cp_async_wait<0>();
+  __syncwarp();
+
+  // The warp's partial over its ring: [head][D] normalised, then [head] lse.
+  float* part = reinterpret_cast<float*>(hkb_smem + warp * P::RING_SMEM);
+  P::end(st, lane, nh, vs, part, part + HEADS * D);
+  // a NaN among the scores makes the sum NaN: the partial says so instead of counting as empty
+#pragma unroll
+  for (int nt = 0; nt < HEADS / 8; ++nt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const unsigned bad = __ballot_sync(0xffffffffu, st.l[nt][c] != st.l[nt][c]);
+      const int h = nt * 8 + 2 * (lane & 3) + c;
+      if ((lane >> 2) == 0 && h < nh && (bad & (0x11111111u << (lane & 3)))) part[HEADS * D + h] = NAN;
+    }
+  cluster_sync();
+
+  // Fold: a quad of output columns a thread, over all workers' partials.
+  const uint32_t mem = smem_u32(hkb_smem);
+  const int quads = nh * (D / 4), share = (quads + ctas - 1) / ctas;
+  const int x1 = min(quads, (rank + 1) * share);
+  for (int x = rank * share + threadIdx.x; x < x1; x += WARPS * 32) {
+    const int h = x / (D / 4), c = x % (D / 4);
+    float mx = -INFINITY;
+    for (int r = 0; r < ctas; ++r)
+      for (int w = 0; w < WARPS; ++w) mx = fmaxf(mx, peer_f1(peer_smem(mem + w * P::RING_SMEM + (HEADS * D + h) * 4, r)));
+    float den = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = 0; r < ctas; ++r)
+      for (int w = 0; w < WARPS; ++w) {
+        const uint32_t at = peer_smem(mem + w * P::RING_SMEM, r);
+        const float lse = peer_f1(at + (HEADS * D + h) * 4);
+        const float wt = lse == -INFINITY ? 0.f : fast_exp2((lse - mx) * LOG2E);
+        const float4 v = peer_f4(at + (h * D + c * 4) * 4);
+        den += wt;
+        acc.x = fmaf(wt, v.x, acc.x); acc.y = fmaf(wt, v.y, acc.y); acc.z = fmaf(wt, v.z, acc.z); acc.w = fmaf(wt, v.w, acc.w);
+      }
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    uint2 o;
+    o.x = pack16x2<F16>(acc.x * inv, acc.y * inv);
+    o.y = pack16x2<F16>(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(a.d.out + (int64_t)row * a.d.out_stride_tok + (int64_t)(hq0 + h) * a.d.out_stride_head + c * 4) = o;
+    if (a.out_lse && c == 0)
+      a.out_lse[(int64_t)row * a.d.num_q_heads + hq0 + h] = den == 0.f ? -INFINITY : mx + logf(den);
+  }
+  cluster_sync();                // no CTA leaves while a peer reads its memory
+}
+
+template <class P, int WARPS, bool F16>
+static int launch_sparse(const SparseArgs& a, int rows, int splits, cudaStream_t st) {
+  auto kernel = sparse_kernel<P, WARPS, F16>;
+  constexpr int smem = WARPS * P::RING_SMEM;
+  static bool armed[64] = {};    // more than 48 KB of shared memory: asked for once a device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev >= 0 && dev < 64 && !armed[dev]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) armed[dev] = true;
+  }
+  if (e != cudaSuccess) { (void)cudaGetLastError(); hkb_tls_cuda_error = (int)e; return HKB_ERR_CUDA; }
+  return launch_cluster((const void*)kernel, dim3(splits, a.d.num_kv_heads, rows), WARPS * 32, splits, smem, &a, st);
+}
+
+template <int D, bool F16>
+static int dispatch_sparse16(const SparseArgs& a, int rows, int splits, cudaStream_t st) {
+  constexpr int NST = D == 256 ? 2 : 3;
+  if (a.d.group <= 8) return launch_sparse<WalkMMA<D, false, 1, 4, NST, F16>, 4, F16>(a, rows, splits, st);
+  return launch_sparse<WalkMMA<D, false, 2, 4, NST, F16>, 4, F16>(a, rows, splits, st);
+}
+template <int D>
+static int dispatch_sparse8(const SparseArgs& a, int rows, int splits, cudaStream_t st) {
+  if (a.d.group <= 8) return launch_sparse<WalkMMAF8<D, 1, 3, 1>, 4, false>(a, rows, splits, st);
+  return launch_sparse<WalkMMAF8<D, 2, 3, 1>, 4, false>(a, rows, splits, st);
+}
+
+// How many CTAs share a (row, kv head).
+static int sparse_splits(int rows, int kv_heads, int64_t tiles) {
+  int sms = hkb_sm_count(-1);
+  if (sms <= 0) sms = 148;
+  int c = 1;
+  while (c < 8 && (int64_t)rows * kv_heads * c < 2 * sms && tiles > c * 8) c *= 2;
+  return c;
+}
+
+}  // namespace hkb
+
+extern "C" int hkb_paged_sparse_decode(void* out, int64_t out_stride_tok, int64_t out_stride_head, float* out_lse,
+                                       const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+                                       hkb_cache_t kc, hkb_cache_t vc, const int32_t* block_table, int64_t table_stride,
+                                       int max_pages, const int32_t* seq_lens, const int32_t* pages,
+                                       int64_t pages_stride_row, int64_t pages_stride_head, int budget, int num_rows,
+                                       int num_q_heads, int num_kv_heads, int head_dim, int block_size, float scale,
+                                       int kv_dtype, const float* k_scale, const float* v_scale, void* stream) {
+  using namespace hkb;
+  if (num_rows < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || max_pages < 0 || budget < 0) return HKB_ERR_SIZE;
+  if (num_rows == 0) return HKB_OK;
+  if (num_rows > 65535 || num_kv_heads > 65535) return HKB_ERR_SIZE;
+  if (!out || !q || !kc.ptr || !vc.ptr || !seq_lens) return HKB_ERR_NULL;
+  if ((max_pages > 0 && !block_table) || (budget > 0 && !pages)) return HKB_ERR_NULL;
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return HKB_ERR_HEAD_DIM;
+  if (block_size <= 0 || block_size % TILE_TOKENS) return HKB_ERR_BLOCK_SIZE;
+  if (num_q_heads % num_kv_heads || num_q_heads / num_kv_heads > HKB_MAX_GROUP) return HKB_ERR_GROUP;
+  if (kv_dtype != HKB_KV_BF16 && kv_dtype != HKB_KV_FP8_E4M3 && kv_dtype != HKB_KV_F16) return HKB_ERR_DTYPE;
+  const bool fp8 = kv_dtype == HKB_KV_FP8_E4M3;
+  if (fp8 && (!k_scale || !v_scale)) return HKB_ERR_SCALE;
+  if (kc.num_blocks < 1 || vc.num_blocks < 1) return HKB_ERR_SIZE;
+  if ((int64_t)budget * (block_size / TILE_TOKENS) > 0x7fffffff) return HKB_ERR_SIZE;
+  const int es = fp8 ? 1 : 2;
+  if ((kc.stride_block | kc.stride_token | kc.stride_head | vc.stride_block | vc.stride_token | vc.stride_head) * es % 16)
+    return HKB_ERR_STRIDE;
+  if ((q_stride_tok | q_stride_head) % 8 || (out_stride_tok | out_stride_head) % 4) return HKB_ERR_STRIDE;
+  if (((uintptr_t)kc.ptr | (uintptr_t)vc.ptr | (uintptr_t)q) % 16 || (uintptr_t)out % 8 || (uintptr_t)out_lse % 4) return HKB_ERR_ALIGN;
+  SparseArgs s = {};
+  DecodeArgs& a = s.d;
+  a.out = (__nv_bfloat16*)out; a.out_stride_tok = out_stride_tok; a.out_stride_head = out_stride_head;
+  a.q = (const __nv_bfloat16*)q; a.q_stride_tok = q_stride_tok; a.q_stride_head = q_stride_head;
+  a.k = (const uint8_t*)kc.ptr; a.v = (const uint8_t*)vc.ptr;
+  a.k_stride_block = kc.stride_block * es; a.k_stride_token = kc.stride_token * es; a.k_stride_head = kc.stride_head * es;
+  a.v_stride_block = vc.stride_block * es; a.v_stride_token = vc.stride_token * es; a.v_stride_head = vc.stride_head * es;
+  const int64_t nb = kc.num_blocks < vc.num_blocks ? kc.num_blocks : vc.num_blocks;
+  a.num_blocks = nb > 0x7fffffff ? 0x7fffffff : (int)nb;
+  a.block_table = block_table; a.table_stride = table_stride; a.max_pages = max_pages;
+  a.seq_lens = seq_lens;
+  a.num_q_heads = num_q_heads; a.num_kv_heads = num_kv_heads; a.group = num_q_heads / num_kv_heads;
+  a.tiles_per_page = block_size / TILE_TOKENS; a.block_size = block_size;
+  a.scale = scale; a.k_scale = fp8 ? k_scale : nullptr; a.v_scale = fp8 ? v_scale : nullptr;
+  s.pages = pages; s.p_stride_row = pages_stride_row; s.p_stride_head = pages_stride_head; s.budget = budget;
+  s.out_lse = out_lse;
+  const int splits = sparse_splits(num_rows, num_kv_heads, (int64_t)budget * a.tiles_per_page);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (kv_dtype == HKB_KV_F16) {
+    if (head_dim == 128) return dispatch_sparse16<128, true>(s, num_rows, splits, st);
+    return head_dim == 256 ? dispatch_sparse16<256, true>(s, num_rows, splits, st) : dispatch_sparse16<64, true>(s, num_rows, splits, st);
+  }
+  if (fp8) {
+    if (head_dim == 128) return dispatch_sparse8<128>(s, num_rows, splits, st);
+    return head_dim == 256 ? dispatch_sparse8<256>(s, num_rows, splits, st) : dispatch_sparse8<64>(s, num_rows, splits, st);
+  }
+  if (head_dim == 128) return dispatch_sparse16<128, false>(s, num_rows, splits, st);
+  return head_dim == 256 ? dispatch_sparse16<256, false>(s, num_rows, splits, st) : dispatch_sparse16<64, false>(s, num_rows, splits, st);
+}

@@ -1,0 +1,259 @@
+"""Decode over selected pages of the paged KV cache, and the page bookkeeping under it: the host side.
+
+A long context's decode step need not read the whole cache. `update_page_bounds` keeps a summary of every page (the
+least and the greatest key of each channel), `page_scores` bounds from the summaries the best logit a query can have
+in a page, `select_pages` takes the budget's best pages of every query row and kv head, and `paged_sparse_decode`
+attends to those alone. `advance_tables` builds what all of them read -- block tables, slot mapping, positions -- on
+the GPU from the requests' lengths. A step of a layer:
+
+    advance_tables(block_tables, seq_lens, new_tokens, free_pages, free_count, block_size, slots, positions, starts, status)
+    reshape_and_cache(key, value, key_cache, value_cache, slots)                     # hk_dsl_b200.ops.paged
+    update_page_bounds(bounds, key_cache, block_tables, seq_lens)
+    page_scores(scores, query, bounds, block_tables, seq_lens, scale, block_size)
+    select_pages(pages, scores, seq_lens, block_size)
+    paged_sparse_decode(out, query, key_cache, value_cache, block_tables, seq_lens, pages, scale)
+
+Caches, queries and tables are those of `hk_dsl_b200.ops.paged`: `(blocks, block_size, kv_heads, head_dim)` views of any
+strides in bf16, fp16 or fp8-e4m3, `(rows, q_heads, head_dim)` queries, int32 tables and lengths, row i of the query
+belonging to row i of the table. Every call is one launch on torch's current stream; it allocates nothing, reads
+nothing back and can be captured into a CUDA graph. There is no fallback: a call the kernels do not take raises.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from ..runtime import lib as _lib
+from .paged import ACT_DTYPES, _FP8_DTYPES, _cache_t, _need_cuda, _scale_ptr, _stream, kv_dtype_code
+
+#: `status` of `advance_tables`
+REQ_OK, REQ_NO_PAGES, REQ_TABLE_FULL, REQ_NO_ROWS = 0, 1, 2, 3
+
+_WHO = "hk.ops.paged_sparse"
+
+
+def _int32(name: str, t: torch.Tensor, dim: int, dtype=torch.int32) -> None:
+    """An index tensor: `dim` axes, the last one contiguous."""
+    if t.dim() != dim or t.dtype != dtype or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise TypeError(f"{_WHO}: {name} is {tuple(t.shape)} {t.dtype} strides {tuple(t.stride())}; "
+                        f"{dim}-dimensional {dtype} with a contiguous last axis needed")
+
+
+def _page_size(block_size: int) -> int:
+    if block_size < 1:
+        raise ValueError(f"{_WHO}: block_size {block_size}: a positive number of tokens")
+    return int(block_size)
+
+
+def _tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, rows: int) -> None:
+    _int32("block_tables", block_tables, 2)
+    _int32("seq_lens", seq_lens, 1)
+    if block_tables.shape[0] < rows or seq_lens.shape[0] < rows:
+        raise ValueError(f"{_WHO}: block_tables {tuple(block_tables.shape)} and seq_lens {tuple(seq_lens.shape)} "
+                         f"for {rows} rows")
+
+
+def page_bounds(key_cache: torch.Tensor) -> torch.Tensor:
+    """The summary tensor of a key cache: `(blocks, kv_heads, 2, head_dim)` of the cache's type, least keys then
+    greatest, uninitialised (`update_page_bounds` fills the pages that it is told of)."""
+    nb, _, hkv, d = key_cache.shape
+    return torch.empty(nb, hkv, 2, d, device=key_cache.device, dtype=key_cache.dtype)
+
+
+def advance_tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, new_tokens: torch.Tensor,
+                   free_pages: torch.Tensor, free_count: torch.Tensor, block_size: int, slot_mapping: torch.Tensor,
+                   positions: torch.Tensor, query_start_loc: torch.Tensor, status: torch.Tensor) -> None:
+    """Grow or shrink every request by `new_tokens` and write down where its new tokens go; in place, one launch.
+
+    `block_tables` (requests, max_pages) int32 and `seq_lens` (requests,) int32 are the requests as they are;
+    `new_tokens` (requests,) int32 what they ask for: a negative number gives tokens back from the end (rejected
+    drafts), all of them when the request is finished. `free_pages` (pool,) int32 is a stack whose first `free_count`
+    (1,) int32 entries are free pages; new pages come from its top in request order, pages given back go on top of what
+    is left, for the next call. Written: `query_start_loc` (requests + 1,) int32, where each request's new tokens begin;
+    `slot_mapping` and `positions` (rows,) int64 of every new token in that order, -1 and 0 in the rows behind the last
+    one (`reshape_and_cache` skips them, so a captured step may have spare rows); `status` (requests,) int32. A request
+    with `REQ_NO_PAGES` (too few free pages; once one is short, so is every later one that needs any), `REQ_TABLE_FULL`
+    or `REQ_NO_ROWS` keeps its length, gets no page, and its rows get slot -1. A page belongs to one request."""
+    n = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
+    _int32("block_tables", block_tables, 2)
+    for name, t in (("seq_lens", seq_lens), ("new_tokens", new_tokens), ("free_pages", free_pages),
+                    ("free_count", free_count), ("query_start_loc", query_start_loc), ("status", status)):
+        _int32(name, t, 1)
+    _int32("slot_mapping", slot_mapping, 1, torch.int64)
+    _int32("positions", positions, 1, torch.int64)
+    if block_tables.shape[0] < n or new_tokens.shape[0] < n or status.shape[0] < n or query_start_loc.shape[0] < n + 1:
+        raise ValueError(f"{_WHO}: {n} requests (seq_lens) with block_tables {tuple(block_tables.shape)}, new_tokens "
+                         f"{tuple(new_tokens.shape)}, status {tuple(status.shape)}, query_start_loc "
+                         f"{tuple(query_start_loc.shape)} ({n + 1} needed)")
+    if free_count.numel() < 1 or positions.shape[0] != slot_mapping.shape[0]:
+        raise ValueError(f"{_WHO}: free_count holds {free_count.numel()} numbers (1 needed); slot_mapping "
+                         f"{tuple(slot_mapping.shape)} and positions {tuple(positions.shape)} must be alike")
+    if n > 1 and block_tables.stride(0) < block_tables.shape[1]:
+        raise ValueError(f"{_WHO}: block_tables' rows overlap (strides {tuple(block_tables.stride())}); it is written")
+    _need_cuda(block_tables, seq_lens, new_tokens, free_pages, free_count, slot_mapping, positions, query_start_loc, status)
+    _lib.check("hkb_advance_tables", _lib.load().hkb_advance_tables(
+        block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(),
+        new_tokens.data_ptr(), n, _page_size(block_size), free_pages.data_ptr(), free_pages.shape[0],
+        free_count.data_ptr(), slot_mapping.data_ptr(), positions.data_ptr(), slot_mapping.shape[0],
+        query_start_loc.data_ptr(), status.data_ptr(), _stream(seq_lens)))
+
+
+def _kind(cache: torch.Tensor) -> int:
+    code = {torch.bfloat16: _lib.KV_BF16, torch.float16: _lib.KV_F16}.get(cache.dtype)
+    if code is None:
+        if cache.dtype not in _FP8_DTYPES:
+            raise TypeError(f"{_WHO}: a key cache of {cache.dtype} (bfloat16, float16 and float8_e4m3fn, or uint8 for "
+                            f"the latter's bytes, are implemented)")
+        code = _lib.KV_FP8_E4M3
+    return code
+
+
+def _check_bounds(bounds: torch.Tensor) -> None:
+    if bounds.dim() != 4 or bounds.shape[2] != 2 or bounds.stride(3) != 1 or bounds.stride(2) != bounds.shape[3]:
+        raise ValueError(f"{_WHO}: bounds is {tuple(bounds.shape)} strides {tuple(bounds.stride())}; "
+                         f"(blocks, kv_heads, 2, head_dim) with the last two axes contiguous needed (page_bounds)")
+
+
+def update_page_bounds(bounds: torch.Tensor, key_cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                       query_start_loc: Optional[torch.Tensor] = None, *, num_tokens: Optional[int] = None) -> torch.Tensor:
+    """Summarise the pages that hold each sequence's newest tokens: `bounds[b, h, 0]` and `[b, h, 1]` become the least
+    and the greatest key of every channel over the page's tokens below the sequence's length.
+
+    To be called behind the cache write. Without `query_start_loc` every sequence has one new token; with it (int32,
+    sequences + 1, from `advance_tables`) sequence i has `query_start_loc[i + 1] - query_start_loc[i]`, and `num_tokens`, a
+    host number, is at least its last entry (the step's rows). A sequence without new tokens has its last page summarised
+    again: it holds fewer tokens if the sequence was shortened. `bounds` is of the cache's type: nothing is rounded. Pages
+    are read from the cache as it is, so a call may be repeated; sequences of length 0 are left out."""
+    if key_cache.dim() != 4 or key_cache.stride(3) != 1:
+        raise ValueError(f"{_WHO}: key_cache {tuple(key_cache.shape)} strides {tuple(key_cache.stride())}; "
+                         f"(blocks, block_size, kv_heads, head_dim) with head_dim contiguous needed")
+    _check_bounds(bounds)
+    nb, page, hkv, d = key_cache.shape
+    code = _kind(key_cache)
+    if bounds.dtype != key_cache.dtype or bounds.shape[1] != hkv or bounds.shape[3] != d:
+        raise ValueError(f"{_WHO}: bounds {tuple(bounds.shape)} {bounds.dtype} beside a key cache {tuple(key_cache.shape)} "
+                         f"{key_cache.dtype}")
+    n = seq_lens.shape[0]
+    _tables(block_tables, seq_lens, n)
+    if query_start_loc is not None:
+        _int32("query_start_loc", query_start_loc, 1)
+        if query_start_loc.shape[0] < n + 1:
+            raise ValueError(f"{_WHO}: query_start_loc has {query_start_loc.shape[0]} entries for {n} sequences")
+        if num_tokens is None or num_tokens < 0:
+            raise ValueError(f"{_WHO}: query_start_loc needs num_tokens, the rows of the step (a host number), not {num_tokens}")
+    _need_cuda(bounds, key_cache, block_tables, seq_lens, query_start_loc)
+    _lib.check("hkb_page_bounds", _lib.load().hkb_page_bounds(
+        bounds.data_ptr(), bounds.stride(0), bounds.stride(1), bounds.shape[0], _cache_t(key_cache),
+        block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(),
+        query_start_loc.data_ptr() if query_start_loc is not None else None, n, num_tokens or 0, hkv, d, page, code,
+        _stream(bounds)))
+    return bounds
+
+
+def _positive(scale: float) -> float:
+    scale = float(scale)
+    if not scale > 0.0:
+        raise ValueError(f"{_WHO}: scale {scale}: the greatest logit is only bounded for a positive one")
+    return scale
+
+
+def _query(name: str, t: torch.Tensor) -> None:
+    if t.dim() != 3 or t.dtype not in ACT_DTYPES or t.stride(2) != 1:
+        raise ValueError(f"{_WHO}: {name} is {tuple(t.shape)} {t.dtype} strides {tuple(t.stride())}; "
+                         f"(rows, q_heads, head_dim) bfloat16 or float16 with head_dim contiguous needed")
+
+
+def page_scores(scores: torch.Tensor, query: torch.Tensor, bounds: torch.Tensor, block_tables: torch.Tensor,
+                seq_lens: torch.Tensor, scale: float, block_size: int, kv_cache_dtype: str = "auto",
+                k_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The bound of the best logit every query row can have in every page of its sequence.
+
+    `scores` (rows, kv_heads, max_pages) fp32 gets `scale * k_scale * max_g sum_d max(q_gd low_d, q_gd high_d)`, the
+    greatest over the kv head's group of query heads, and -inf for the table's columns behind the sequence.
+    `query` (rows, q_heads, head_dim); `bounds` from `update_page_bounds`."""
+    _query("query", query)
+    _check_bounds(bounds)
+    rows, hq, d = query.shape
+    nb, hkv, _, bd = bounds.shape
+    width = block_tables.shape[1] if block_tables.dim() == 2 else 0
+    if bd != d or hkv < 1 or hq % hkv:
+        raise ValueError(f"{_WHO}: query {tuple(query.shape)} beside bounds {tuple(bounds.shape)}")
+    if scores.dtype != torch.float32 or tuple(scores.shape) != (rows, hkv, width) or (width > 1 and scores.stride(2) != 1):
+        raise ValueError(f"{_WHO}: scores is {tuple(scores.shape)} {scores.dtype}; ({rows}, {hkv}, {width}) float32 with "
+                         f"contiguous columns needed (the table's width)")
+    _tables(block_tables, seq_lens, rows)
+    code = kv_dtype_code(kv_cache_dtype, bounds, query.dtype)
+    fp8 = code == _lib.KV_FP8_E4M3
+    scale = _positive(scale)
+    _need_cuda(scores, query, bounds, block_tables, seq_lens, k_scale)
+    _lib.check("hkb_page_scores", _lib.load().hkb_page_scores(
+        scores.data_ptr(), scores.stride(0), scores.stride(1), width, query.data_ptr(), query.stride(0), query.stride(1),
+        bounds.data_ptr(), bounds.stride(0), bounds.stride(1), nb, block_tables.data_ptr(), block_tables.stride(0),
+        seq_lens.data_ptr(), rows, hq, hkv, d, _page_size(block_size), scale, code,
+        _scale_ptr(k_scale, fp8, "k_scale"), _stream(query)))
+    return scores
+
+
+def select_pages(pages: torch.Tensor, scores: torch.Tensor, seq_lens: torch.Tensor, block_size: int, *,
+                 first: int = 1, last: int = 4) -> torch.Tensor:
+    """The budget's best pages: `pages` (rows, kv_heads, budget) int32 gets, in ascending order and -1 behind, the
+    `first` and the `last` pages of the row's sequence and then those of the greatest `scores` (rows, kv_heads, columns)
+    fp32, ties to the lowest page, NaN above all numbers. A row with no more pages than the budget gets them all.
+    The entries number the row's pages (columns of its block table), as `paged_sparse_decode` reads them."""
+    _int32("pages", pages, 3)
+    _int32("seq_lens", seq_lens, 1)
+    rows, hkv, budget = pages.shape
+    if scores.dtype != torch.float32 or scores.dim() != 3 or tuple(scores.shape[:2]) != (rows, hkv) \
+            or (scores.shape[2] > 1 and scores.stride(2) != 1):
+        raise ValueError(f"{_WHO}: scores is {tuple(scores.shape)} {scores.dtype} beside pages {tuple(pages.shape)}; "
+                         f"({rows}, {hkv}, columns) float32 with contiguous columns needed")
+    if seq_lens.shape[0] < rows:
+        raise ValueError(f"{_WHO}: {seq_lens.shape[0]} lengths for {rows} rows")
+    if first < 0 or last < 0 or first + last > budget:
+        raise ValueError(f"{_WHO}: first {first} and last {last} pages of a budget of {budget}")
+    _need_cuda(pages, scores, seq_lens)
+    _lib.check("hkb_select_pages", _lib.load().hkb_select_pages(
+        pages.data_ptr(), pages.stride(0), pages.stride(1), budget, scores.data_ptr(), scores.stride(0), scores.stride(1),
+        scores.shape[2], seq_lens.data_ptr(), rows, hkv, _page_size(block_size), first, last, _stream(pages)))
+    return pages
+
+
+def paged_sparse_decode(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                        block_tables: torch.Tensor, seq_lens: torch.Tensor, pages: torch.Tensor, scale: float,
+                        kv_cache_dtype: str = "auto", k_scale: Optional[torch.Tensor] = None,
+                        v_scale: Optional[torch.Tensor] = None, *, out_lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Decode attention of one query token a row over the row's selected pages: `paged_attention_decode` where row r
+    and kv head h see only the tokens of `pages[r, h]` (int32 (rows, kv_heads, budget), numbers of the sequence's pages;
+    negative entries and pages past the sequence are none) that lie below `seq_lens[r]`. A page listed twice counts
+    twice. With nothing left a row answers zeros. `out_lse` (rows, q_heads) fp32 gets the natural-log sum-exp of the
+    scaled scores (-inf for nothing), so that answers over disjoint pages can be merged (`merge_partials`). A NaN among
+    a row's visible keys, or a logit outside fp32's range, makes the heads that meet it NaN."""
+    _query("query", query)
+    if out.shape != query.shape or out.dtype != query.dtype or out.stride(2) != 1:
+        raise ValueError(f"{_WHO}: out is {tuple(out.shape)} {out.dtype}; it must match query {tuple(query.shape)} {query.dtype}")
+    rows, hq, d = query.shape
+    if key_cache.dim() != 4 or value_cache.shape != key_cache.shape or key_cache.stride(3) != 1 or value_cache.stride(3) != 1 \
+            or key_cache.shape[3] != d or value_cache.dtype != key_cache.dtype:
+        raise ValueError(f"{_WHO}: key_cache {tuple(key_cache.shape)} {key_cache.dtype} / value_cache "
+                         f"{tuple(value_cache.shape)} {value_cache.dtype}; two (blocks, block_size, kv_heads, {d}) views "
+                         f"of one dtype needed")
+    _, page, hkv, _ = key_cache.shape
+    _tables(block_tables, seq_lens, rows)
+    _int32("pages", pages, 3)
+    if tuple(pages.shape[:2]) != (rows, hkv):
+        raise ValueError(f"{_WHO}: pages is {tuple(pages.shape)}; ({rows}, {hkv}, budget) needed")
+    if out_lse is not None and (out_lse.dtype != torch.float32 or tuple(out_lse.shape) != (rows, hq) or not out_lse.is_contiguous()):
+        raise ValueError(f"{_WHO}: out_lse is {tuple(out_lse.shape)} {out_lse.dtype}; contiguous ({rows}, {hq}) float32 needed")
+    code = kv_dtype_code(kv_cache_dtype, key_cache, query.dtype)
+    fp8 = code == _lib.KV_FP8_E4M3
+    scale = _positive(scale)
+    _need_cuda(out, query, key_cache, value_cache, block_tables, seq_lens, pages, k_scale, v_scale, out_lse)
+    _lib.check("hkb_paged_sparse_decode", _lib.load().hkb_paged_sparse_decode(
+        out.data_ptr(), out.stride(0), out.stride(1), out_lse.data_ptr() if out_lse is not None else None,
+        query.data_ptr(), query.stride(0), query.stride(1), _cache_t(key_cache), _cache_t(value_cache),
+        block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(),
+        pages.data_ptr(), pages.stride(0), pages.stride(1), pages.shape[2], rows, hq, hkv, d, page, scale, code,
+        _scale_ptr(k_scale, fp8, "k_scale"), _scale_ptr(v_scale, fp8, "v_scale"), _stream(query)))
+    return out

@@ -97,6 +97,18 @@ SIGNATURES = {
     "hkb_prefill_tc_error": (c_int, [c_int]),
     "hkb_merge": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
                           c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "hkb_advance_tables": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_void_p,
+                                   c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
+    "hkb_page_bounds": (c_int, [c_void_p, c_int64, c_int64, c_int64, CacheT, c_void_p, c_int64, c_int, c_void_p, c_void_p,
+                                c_int, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
+    "hkb_page_scores": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
+                                c_void_p, c_void_p]),
+    "hkb_select_pages": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int,
+                                 c_int, c_int, c_int, c_int, c_void_p]),
+    "hkb_paged_sparse_decode": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, CacheT, CacheT,
+                                        c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int64, c_int,
+                                        c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_void_p]),
     "hkb_walk_uses_mma": (c_int, [c_int, c_int]),
     "hkb_plan_splits": (c_int, [c_int, c_int, c_int, c_int]),
     "hkb_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),

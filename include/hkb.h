@@ -452,6 +452,93 @@ int hkb_paged_decode_static(void* out, int64_t out_stride_tok, int64_t out_strid
                             int num_splits, void* stream);
 
 /*
+ * Block tables, slots and positions of a step from request lengths, on the device and in place. Request i of
+ * num_reqs holds seq_lens[i] tokens (negative counts as 0) in pages of block_size and asks for new_tokens[i]
+ * more; a negative value gives that many back from its end (rejected drafts; a whole length: a finished
+ * request). Free pages are the stack free_pages[0 .. *free_count).
+ *   - q_start[i], num_reqs + 1 entries: where the request's new tokens begin among the step's rows, in request order.
+ *   - slot_mapping[t], positions[t] (int64, num_rows entries): row t's slot page * block_size + offset and its
+ *     position. Rows behind the last request's: slot -1, position 0. (hkb_reshape_and_cache skips slot -1.)
+ *   - status[i]: HKB_REQ_*. A refused request keeps its length and gets no page; its rows get slot -1.
+ *   - block_table rows of growing requests are extended; pages come from the stack's top, in request order, and
+ *     pages given back go on the stack behind them, also in request order: they are there for the next call. Once a
+ *     request finds too few pages, so do all behind it that need any. Entries past a request's pages stay as they were.
+ *   - seq_lens and *free_count are updated.
+ * A page belongs to one request; the stack's capacity must hold all pages that can be free at once (what does not
+ * fit is dropped). Deterministic. A call that runs beside another on the same arrays races with it.
+ *
+ * Stands beside the engine's own host-side scheduler state, which the reference reads as built
+ * (python/hk/integration/vllm_backend.py:582-599: slot_mapping, block_table, seq_lens from vLLM).
+ */
+#define HKB_REQ_OK 0
+#define HKB_REQ_NO_PAGES 1    /* too few free pages */
+#define HKB_REQ_TABLE_FULL 2  /* more pages than the block table has columns, or more than 2^31 - 1 tokens */
+#define HKB_REQ_NO_ROWS 3     /* its rows end behind num_rows */
+int hkb_advance_tables(int32_t* block_table, int64_t table_stride, int max_pages, int32_t* seq_lens,
+                       const int32_t* new_tokens, int num_reqs, int block_size,
+                       int32_t* free_pages, int64_t free_capacity, int32_t* free_count,
+                       int64_t* slot_mapping, int64_t* positions, int64_t num_rows,
+                       int32_t* q_start, int32_t* status, void* stream);
+
+/*
+ * Page summaries for a decode over selected pages: bounds[b, h, 0, :] and bounds[b, h, 1, :] become the least and
+ * the greatest key of every channel of kv head h over the tokens of page b below its sequence's length. Of
+ * sequence i the pages that hold its last max(1, q_start[i+1] - q_start[i]) tokens are summarised (q_start NULL: its
+ * last token), from the cache as it is: call it behind the cache write of those tokens. A sequence without new tokens
+ * has its last page summarised again, which holds fewer tokens if the sequence was shortened. bounds has the cache's element type (values are kept exactly, fp8 ones as stored); its last two axes
+ * are contiguous, head_dim each. A NaN key makes the channel's bounds NaN. Page ids outside
+ * [0, min(bounds_blocks, k_cache.num_blocks)) are skipped. num_tokens: an upper bound of q_start[num_seqs], which
+ * must not be below it. block_size is any positive number.
+ */
+int hkb_page_bounds(void* bounds, int64_t bounds_stride_block, int64_t bounds_stride_head, int64_t bounds_blocks,
+                    hkb_cache_t k_cache, const int32_t* block_table, int64_t table_stride, int max_pages,
+                    const int32_t* seq_lens, const int32_t* q_start, int num_seqs, int64_t num_tokens,
+                    int num_kv_heads, int head_dim, int block_size, int kv_dtype, void* stream);
+
+/*
+ * Page scores: scores[r, h, p] = scale * k_scale * max over the query heads g of kv head h of
+ * sum_d max(q[r, g, d] * low_d, q[r, g, d] * high_d), low and high from page block_table[r, p]'s summary: no key
+ * between them has a greater logit. Computed as max(q, 0) . high + min(q, 0) . low in fp32 (an infinite bound that
+ * meets a zero gives NaN). Pages at or past ceil(seq_lens[r] / block_size) get -inf, in all num_columns columns of
+ * the table. A NaN among a page's products makes its score NaN. q is bf16 (fp16 with HKB_KV_F16); scores fp32 with
+ * contiguous columns; k_scale as in hkb_paged_decode.
+ */
+int hkb_page_scores(float* scores, int64_t scores_stride_row, int64_t scores_stride_head, int num_columns,
+                    const void* q, int64_t q_stride_row, int64_t q_stride_head,
+                    const void* bounds, int64_t bounds_stride_block, int64_t bounds_stride_head, int64_t bounds_blocks,
+                    const int32_t* block_table, int64_t table_stride, const int32_t* seq_lens,
+                    int num_rows, int num_q_heads, int num_kv_heads, int head_dim, int block_size, float scale,
+                    int kv_dtype, const float* k_scale, void* stream);
+
+/*
+ * The budget's best pages of every (row, kv head). Row r has n = min(ceil(seq_lens[r] / block_size), num_columns)
+ * pages; its first `first` and last `last` pages are taken, then those of the greatest scores (ties to the lowest
+ * page, NaN above all numbers), min(n, budget) in all. pages[r, h, :] gets them in ascending order, -1 behind.
+ * first + last <= budget. Columns at or past n are not read.
+ */
+int hkb_select_pages(int32_t* pages, int64_t pages_stride_row, int64_t pages_stride_head, int budget,
+                     const float* scores, int64_t scores_stride_row, int64_t scores_stride_head, int num_columns,
+                     const int32_t* seq_lens, int num_rows, int num_kv_heads, int block_size, int first, int last,
+                     void* stream);
+
+/*
+ * Decode attention over selected pages: hkb_paged_decode (one new token a row, the caches, dtypes, head sizes and
+ * groups of that call) where query row r and kv head h read only the pages pages[r, h, 0 .. budget) of row r's
+ * sequence (numbers of its block-table row, not page ids), and of those only tokens below seq_lens[r]. A negative
+ * entry, or one past the sequence or max_pages, is no page; a page that is listed twice counts twice. A row that is
+ * left with nothing answers zeros and, if out_lse (fp32, (rows, q heads)) is not NULL, -inf; otherwise out_lse gets
+ * the natural-log sum-exp of the scaled scores, so the answer can be merged with another (hkb_merge). scale and
+ * k_scale must be positive. One launch, no scratch. out is 8-byte aligned, with strides that are multiples of 4.
+ */
+int hkb_paged_sparse_decode(void* out, int64_t out_stride_tok, int64_t out_stride_head, float* out_lse,
+                            const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+                            hkb_cache_t k_cache, hkb_cache_t v_cache,
+                            const int32_t* block_table, int64_t table_stride, int max_pages, const int32_t* seq_lens,
+                            const int32_t* pages, int64_t pages_stride_row, int64_t pages_stride_head, int budget,
+                            int num_rows, int num_q_heads, int num_kv_heads, int head_dim, int block_size, float scale,
+                            int kv_dtype, const float* k_scale, const float* v_scale, void* stream);
+
+/*
  * Split planner: how many ways to cut the KV axis so that num_seqs*num_kv_heads
  * CTAs fill sm_count SMs; a power of two, at most max_tiles (16-token tiles of
  * the longest sequence the engine allows) and HKB_MAX_SPLITS. A function of host
