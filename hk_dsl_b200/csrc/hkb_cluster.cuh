@@ -41,7 +41,8 @@ __device__ __forceinline__ float peer_f1(uint32_t addr) {
   return v;
 }
 
-// One argument struct, `cluster` CTAs of grid.x a cluster (1: an ordinary launch; up to 8, the portable size).
+// One argument struct, `cluster` CTAs of grid.x a cluster (1: an ordinary launch; past 8, the portable size,
+// the kernel has to be allowed to).
 inline int launch_cluster(const void* kernel, dim3 grid, int threads, int cluster, int smem_bytes, const void* args, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;

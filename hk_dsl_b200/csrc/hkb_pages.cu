@@ -16,13 +16,12 @@ namespace hkb {
 // (tokens, pages taken, pages given) place everything: token t belongs to the request whose range of the first
 // sum holds t, a new page comes from position count - 1 - (second sum) of the free stack, a page given back
 // goes to position count - taken + (third sum). No request waits for another, so one cluster does it all:
-// every CTA scans all requests (a trip to memory a CHUNK of them), then takes its share of the tokens and
-// pages; the in-place updates -- the stack's top, the lengths, the count -- come after a cluster barrier, when
-// every CTA has read what it needs of the old state. Deterministic: no atomics.
-// Bound: latency (two dependent trips and the scans), then the stores of 16 bytes a token.
+// every CTA scans all requests (a chunk of CHUNK at a time: one trip to memory and one three-fold scan), then takes
+// its share of the tokens and pages; the in-place updates -- the stack's top, the lengths, the count -- come after a
+// cluster barrier, when every CTA has read what it needs of the old state. Deterministic: no atomics.
+// Bound: latency (the scan, then two dependent trips), then the stores of 16 bytes a token.
 // ---------------------------------------------------------------------------------
-constexpr int ADV_THREADS = 512;      // requests a chunk, one a thread
-constexpr int ADV_WARPS = ADV_THREADS / 32;
+constexpr int ADV_BLOCKS = 2;                     // 32-token blocks a warp looks up at once
 
 struct AdvanceArgs {
   int* table;
@@ -31,6 +30,8 @@ struct AdvanceArgs {
   int* seq_lens;
   const int* new_tokens;
   int num_reqs, page;
+  uint32_t page_magic;             // pos / page = umulhi(pos, magic) >> shift for pos < 2^31, page > 1:
+  int page_shift;                  // magic = floor(2^(31 + l) / page) + 1, shift = l - 1, l = ceil(log2 page)
   int* free_pages;
   int* free_count;
   int64_t free_cap;
@@ -41,153 +42,261 @@ struct AdvanceArgs {
   int* status;
 };
 
-// Inclusive sum over the CTA's threads (in thread order); `sums` is one value a warp, reused call by call.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sums, int64_t& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int x = 1; x < 32; x <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, v, x);
-    if (lane >= x) v += y;
-  }
-  __syncthreads();                       // `sums` of the call before is read
-  if (lane == 31) sums[warp] = v;
-  __syncthreads();
-  int64_t before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < ADV_WARPS; ++w) {
-    const int64_t s = sums[w];
-    if (w < warp) before += s;
-    total += s;
-  }
-  return v + before;
+// Sums are held at 2^31 - 1 (adding without going over is associative): no token, page or start past that is real.
+struct Sums { int tokens, need, give; };
+__device__ __forceinline__ int clamp31(int64_t x) { return (int)max(min(x, (int64_t)0x7fffffff), (int64_t)0); }
+__device__ __forceinline__ int sat_add(int x, int y) { return (int)min((uint32_t)x + (uint32_t)y, 0x7fffffffu); }
+__device__ __forceinline__ Sums operator+(const Sums& x, const Sums& y) {
+  return {sat_add(x.tokens, y.tokens), sat_add(x.need, y.need), sat_add(x.give, y.give)};
+}
+__device__ __forceinline__ Sums shfl_up(const Sums& s, int by) {
+  return {__shfl_up_sync(0xffffffffu, s.tokens, by), __shfl_up_sync(0xffffffffu, s.need, by), __shfl_up_sync(0xffffffffu, s.give, by)};
+}
+__device__ __forceinline__ Sums shfl_at(const Sums& s, int lane) {
+  return {__shfl_sync(0xffffffffu, s.tokens, lane), __shfl_sync(0xffffffffu, s.need, lane), __shfl_sync(0xffffffffu, s.give, lane)};
 }
 
-// The first of n ascending inclusive sums that is greater than x: the thread whose range holds x.
-__device__ __forceinline__ int range_of(const int64_t* ends, int n, int64_t x) {
-  int lo = 0, hi = n - 1;
+// What a chunk of requests comes to, in shared memory; sums are inclusive and relative to the chunk's beginning.
+template <int WARPS, int EACH>
+struct AdvChunk {
+  static constexpr int CHUNK = WARPS * 32 * EACH;
+  int ends[CHUNK], upto[CHUNK], gives[CHUNK];     // tokens, pages taken, pages given
+  int old[CHUNK], have[CHUNK];                    // have < 0: refused (-1 - pages)
+  Sums warp[WARPS];
+};
+
+struct AdvRequest { int64_t old, grow, have, want; int status; };
+
+__device__ __forceinline__ AdvRequest adv_request(const AdvanceArgs& a, int r) {
+  AdvRequest q = {0, 0, 0, 0, HKB_REQ_OK};
+  if (r < a.num_reqs) { q.old = max(a.seq_lens[r], 0); q.grow = a.new_tokens[r]; }
+  const int64_t after = max(q.old + q.grow, (int64_t)0);
+  q.have = min((int64_t)(((uint32_t)q.old + (uint32_t)a.page - 1u) / (uint32_t)a.page), (int64_t)a.max_pages);
+  q.want = (int64_t)(((uint32_t)after + (uint32_t)a.page - 1u) / (uint32_t)a.page);     // old, grow < 2^31
+  if (after > 0x7fffffff) q.want = (int64_t)a.max_pages + 1;
+  return q;
+}
+
+// Inclusive sums of this thread's EACH requests, in request order, and the chunk's totals.
+template <int WARPS, int EACH>
+__device__ __forceinline__ void adv_scan(AdvChunk<WARPS, EACH>& c, const Sums (&v)[EACH], Sums (&incl)[EACH], Sums& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Sums none = {0, 0, 0};
+  incl[0] = v[0];
+#pragma unroll
+  for (int e = 1; e < EACH; ++e) incl[e] = incl[e - 1] + v[e];
+  Sums s = incl[EACH - 1];
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    const Sums y = shfl_up(s, x);
+    if (lane >= x) s = s + y;
+  }
+  __syncthreads();                                // the chunk before is done with
+  if (lane == 31) c.warp[warp] = s;
+  __syncthreads();
+  Sums w = lane < WARPS ? c.warp[lane] : none;    // every warp scans the warps' sums
+#pragma unroll
+  for (int x = 1; x < WARPS; x <<= 1) {
+    const Sums y = shfl_up(w, x);
+    if (lane >= x) w = w + y;
+  }
+  total = shfl_at(w, WARPS - 1);
+  const Sums warps = shfl_at(w, max(warp - 1, 0)), lanes = shfl_up(s, 1);
+  const Sums before = (warp ? warps : none) + (lane ? lanes : none);
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) incl[e] = before + incl[e];
+}
+
+// A chunk's requests: their sums into shared memory, this thread's own into `q`; `before`: the sums of the chunks before.
+template <int WARPS, int EACH>
+__device__ __forceinline__ void adv_chunk(const AdvanceArgs& a, AdvChunk<WARPS, EACH>& c, int c0, int64_t count,
+                                          const Sums& before, Sums& total, AdvRequest (&q)[EACH]) {
+  Sums v[EACH], incl[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) q[e] = adv_request(a, c0 + threadIdx.x * EACH + e);
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    if (q[e].grow > 0 && q[e].want > a.max_pages) q[e].status = HKB_REQ_TABLE_FULL;
+    v[e].tokens = clamp31(q[e].grow);
+    v[e].need = q[e].grow > 0 && q[e].status == HKB_REQ_OK ? clamp31(q[e].want - q[e].have) : 0;
+    v[e].give = q[e].grow < 0 ? clamp31(q[e].have - q[e].want) : 0;
+  }
+  adv_scan(c, v, incl, total);
+  if ((int64_t)before.tokens + total.tokens > a.tokens) {  // some of the rows are missing: those requests take no page either
+#pragma unroll
+    for (int e = 0; e < EACH; ++e)
+      if (q[e].grow > 0 && q[e].status == HKB_REQ_OK && (int64_t)before.tokens + incl[e].tokens > a.tokens) {
+        q[e].status = HKB_REQ_NO_ROWS;
+        v[e].need = 0;
+      }
+    adv_scan(c, v, incl, total);
+  }
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    if (v[e].need > 0 && (int64_t)before.need + incl[e].need > count) q[e].status = HKB_REQ_NO_PAGES;
+    const int i = threadIdx.x * EACH + e;
+    c.ends[i] = incl[e].tokens; c.upto[i] = incl[e].need; c.gives[i] = incl[e].give;
+    c.old[i] = (int)q[e].old;
+    c.have[i] = q[e].status == HKB_REQ_OK ? (int)q[e].have : -1 - (int)q[e].have;
+  }
+  __syncthreads();
+}
+
+// The first of n ascending inclusive sums that is greater than x: the request whose range holds x. lo: none before it is.
+__device__ __forceinline__ int range_of(const int* ends, int lo, int n, int x) {
+  int hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (ends[mid] > x) hi = mid; else lo = mid + 1;
   }
   return lo;
 }
+// The same for an x that the warp shares: 32 candidates at once.
+__device__ __forceinline__ int range_of_warp(const int* ends, int n, int x, int lane) {
+  int lo = 0, hi = n;                             // the answer is in [lo, hi)
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32 | 1, at = lo + (lane + 1) * step - 1;        // odd: 32 different banks
+    const int m = __popc(__ballot_sync(0xffffffffu, at < hi - 1 && ends[at] <= x));   // groups that lie before it
+    lo = lo + m * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
 
-__global__ void __launch_bounds__(ADV_THREADS) advance_kernel(const AdvanceArgs a) {
-  __shared__ int64_t sums[ADV_WARPS];
-  __shared__ int64_t s_ends[ADV_THREADS], s_upto[ADV_THREADS];
-  __shared__ int s_old[ADV_THREADS], s_have[ADV_THREADS], s_ok[ADV_THREADS], s_need[ADV_THREADS];
-  const int tid = threadIdx.x;
+template <int WARPS, int EACH>
+__global__ void __launch_bounds__(WARPS * 32) advance_kernel(const AdvanceArgs a) {
+  __shared__ AdvChunk<WARPS, EACH> c;
+  constexpr int THREADS = WARPS * 32, CHUNK = THREADS * EACH;
+  const int tid = threadIdx.x, lane = tid & 31;
   const int ctas = cluster_size(), rank = cluster_rank();
   const int64_t count = min((int64_t)max(*a.free_count, 0), a.free_cap);
-  const int P = a.page;
+  const uint32_t P = (uint32_t)a.page;
 
-  int64_t tok0 = 0, upto0 = 0, taken = 0, given = 0;      // sums over the chunks before
-  for (int c0 = 0; c0 < a.num_reqs; c0 += ADV_THREADS) {
-    const int n = min(ADV_THREADS, a.num_reqs - c0), r = c0 + tid;
-    int64_t old = 0, grow = 0;
-    if (tid < n) { old = max(a.seq_lens[r], 0); grow = a.new_tokens[r]; }
-    const int64_t after = max(old + grow, (int64_t)0);
-    const int64_t have = min((old + P - 1) / P, (int64_t)a.max_pages), want = (after + P - 1) / P;
-    const int64_t q = max(grow, (int64_t)0);
-    int64_t tok_total, need_total, give_total;
-    const int64_t ends = tok0 + block_scan(q, sums, tok_total);
-    int st = HKB_REQ_OK;
-    if (q > 0) {
-      if (want > a.max_pages || after > 0x7fffffffLL) st = HKB_REQ_TABLE_FULL;
-      else if (ends > a.tokens) st = HKB_REQ_NO_ROWS;
-    }
-    const int64_t need = st == HKB_REQ_OK && q > 0 ? max(want - have, (int64_t)0) : 0;
-    const int64_t upto = upto0 + block_scan(need, sums, need_total);
-    if (need > 0 && upto > count) st = HKB_REQ_NO_PAGES;
-    block_scan(grow < 0 ? max(have - want, (int64_t)0) : 0, sums, give_total);
-    s_ends[tid] = ends; s_upto[tid] = upto;
-    s_old[tid] = (int)old; s_have[tid] = (int)have; s_ok[tid] = st == HKB_REQ_OK; s_need[tid] = (int)need;
-    if (tid < n && (c0 / ADV_THREADS) % ctas == rank) {
-      a.q_start[r + 1] = (int)min(ends, (int64_t)0x7fffffff);
-      if (r == 0) a.q_start[0] = 0;
-      a.status[r] = st;
-    }
-    __syncthreads();
-
-    // this chunk's tokens, shared out over the cluster
-    const int64_t t1 = min(tok0 + tok_total, a.tokens);
-    for (int64_t t = tok0 + rank * ADV_THREADS + tid; t < t1; t += ctas * ADV_THREADS) {
-      const int i = range_of(s_ends, n, t);
-      const int64_t start = i ? s_ends[i - 1] : tok0;
-      const int64_t pos = s_old[i] + (t - start);
-      const int64_t lp = pos / P;
-      int64_t block = -1;
-      if (s_ok[i]) {
-        if (lp < s_have[i]) block = a.table[(int64_t)(c0 + i) * a.table_stride + lp];
-        else block = a.free_pages[count - 1 - (s_upto[i] - s_need[i] + lp - s_have[i])];
+  Sums before = {0, 0, 0}, total;
+  int64_t taken = 0;
+  AdvRequest q[EACH];
+  for (int c0 = 0; c0 < a.num_reqs; c0 += CHUNK) {
+    const int n = min(CHUNK, a.num_reqs - c0);
+    adv_chunk(a, c, c0, count, before, total, q);
+    if ((c0 / CHUNK) % ctas == rank) {
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int i = tid * EACH + e;
+        if (i >= n) continue;
+        a.q_start[c0 + i + 1] = sat_add(before.tokens, c.ends[i]);
+        a.status[c0 + i] = q[e].status;
       }
-      a.slots[t] = block >= 0 ? block * P + (pos - lp * P) : -1;
-      a.positions[t] = pos;
     }
-    // and its new pages. Once one request gets none, none of those after it that need pages gets any (the sum
-    // runs on), so the pages handed out are the sum's first ones, in request order.
-    const int64_t p1 = min(upto0 + need_total, count);
-    for (int64_t x = upto0 + rank * ADV_THREADS + tid; x < p1; x += ctas * ADV_THREADS) {
-      const int i = range_of(s_upto, n, x);
-      if (!s_ok[i]) continue;
-      const int64_t at = s_have[i] + x - (s_upto[i] - s_need[i]);
-      a.table[(int64_t)(c0 + i) * a.table_stride + at] = a.free_pages[count - 1 - x];
+    // This chunk's tokens, dealt to the warps ADV_BLOCKS blocks of 32 at a time (longer runs leave the tokens of many
+    // short requests to a few warps). Where they are all one request's, what they share is looked up once; else every
+    // lane looks its request up, block by block. A new page's first position is one of the new tokens', whose lane also writes the page into the table. Once one request gets none,
+    // none of those after it that need pages gets any (the sum runs on), so the pages handed out are the sum's first
+    // ones, in request order.
+    const int rows = clamp31(min((int64_t)total.tokens, a.tokens - before.tokens));     // of the chunk
+    const int64_t top = count - 1 - before.need;
+    int64_t* const slots = a.slots + before.tokens;
+    int64_t* const positions = a.positions + before.tokens;
+    // one token of request r: its page is table[lp] or, for a new one, last[-lp]
+    auto put = [&](int t, uint32_t pos, int have, int* table, const int* last) {
+      const uint32_t lp = P == 1 ? pos : __umulhi(pos, a.page_magic) >> a.page_shift;
+      const uint32_t off = pos - lp * P;
+      int block = -1;
+      if (have >= 0) {
+        const bool fresh = (int)lp >= have;
+        block = fresh ? last[-(int64_t)lp] : table[lp];
+        if (fresh && off == 0) table[lp] = block;
+      }
+      slots[t] = block >= 0 ? (int64_t)block * P + off : -1;
+      positions[t] = pos;
+    };
+    auto enter = [&](int r, uint32_t& shift_r, int& have_r, int*& table_r, const int*& last_r) {
+      shift_r = (uint32_t)c.old[r] - (uint32_t)(r ? c.ends[r - 1] : 0);
+      have_r = c.have[r];
+      table_r = a.table + (int64_t)(c0 + r) * a.table_stride;
+      last_r = a.free_pages + (top - (r ? c.upto[r - 1] : 0) + have_r);
+    };
+    for (int g0 = (rank * WARPS + (tid >> 5)) * 32 * ADV_BLOCKS; g0 < rows; g0 += ctas * WARPS * 32 * ADV_BLOCKS) {
+      uint32_t shift;                             // position less token
+      int i = range_of_warp(c.ends, n, g0, lane), have;
+      int* table;
+      const int* last;
+      if (g0 + 32 * ADV_BLOCKS <= min(c.ends[i], rows)) {
+        enter(i, shift, have, table, last);
+#pragma unroll
+        for (int u = 0; u < ADV_BLOCKS; ++u) put(g0 + u * 32 + lane, shift + (uint32_t)(g0 + u * 32 + lane), have, table, last);
+        continue;
+      }
+      for (int t0 = g0; t0 < min(g0 + 32 * ADV_BLOCKS, rows); t0 += 32) {
+        const int t = t0 + lane;
+        // the lane's request: among the next 32, a candidate a lane, by bisection over the lanes; else further on
+        const int mine = c.ends[min(i + lane, n - 1)];
+        int r = 0;
+#pragma unroll
+        for (int step = 16; step > 0; step >>= 1)
+          if (__shfl_sync(0xffffffffu, mine, r + step - 1) <= t) r += step;
+        r += __shfl_sync(0xffffffffu, mine, r) <= t;
+        r = min(i + r, n - 1);
+        if (t < rows) {
+          if (c.ends[r] <= t) r = range_of(c.ends, r, n, t);
+          enter(r, shift, have, table, last);
+          put(t, shift + (uint32_t)t, have, table, last);
+        }
+        i = __shfl_sync(0xffffffffu, r, 31);      // where the next block begins, or before
+      }
     }
-    int64_t got;
-    block_scan(s_ok[tid] ? need : 0, sums, got);
-    taken += got;
-    tok0 += tok_total; upto0 += need_total; given += give_total;
-    __syncthreads();
+    const int fresh = clamp31(min((int64_t)total.need, count - before.need));
+    if ((int64_t)before.need + total.need <= count) {
+      taken += total.need;
+    } else if (fresh > 0) {                       // short: up to the last request that fits
+      const int i = range_of(c.upto, 0, n, fresh);          // the first one past the stack
+      taken += i ? c.upto[i - 1] : 0;
+    }
+    before = before + total;
+    // the next adv_scan waits for every thread before it writes
   }
-  for (int64_t t = min(tok0, a.tokens) + rank * ADV_THREADS + tid; t < a.tokens; t += ctas * ADV_THREADS) {
+  for (int64_t t = min((int64_t)before.tokens, a.tokens) + rank * THREADS + tid; t < a.tokens; t += ctas * THREADS) {
     a.slots[t] = -1;
     a.positions[t] = 0;
   }
-  if (a.num_reqs == 0 && rank == 0 && tid == 0) a.q_start[0] = 0;
-  cluster_sync();
+  if (rank == 0 && tid == 0) a.q_start[0] = 0;
+  if (ctas > 1) cluster_sync(); else __syncthreads();
 
-  if (given > 0) {       // the same in every CTA
-    int64_t at0 = count - taken;
-    for (int c0 = 0; c0 < a.num_reqs; c0 += ADV_THREADS) {
-      const int n = min(ADV_THREADS, a.num_reqs - c0), r = c0 + tid;
-      int64_t old = 0, grow = 0;
-      if (tid < n) { old = max(a.seq_lens[r], 0); grow = a.new_tokens[r]; }
-      const int64_t have = min((old + P - 1) / P, (int64_t)a.max_pages);
-      const int64_t want = (max(old + grow, (int64_t)0) + P - 1) / P;
-      const int64_t give = grow < 0 ? max(have - want, (int64_t)0) : 0;
-      int64_t total;
-      s_upto[tid] = block_scan(give, sums, total);
-      s_have[tid] = (int)want; s_need[tid] = (int)give;
-      __syncthreads();
-      for (int64_t x = rank * ADV_THREADS + tid; x < total; x += ctas * ADV_THREADS) {
-        const int i = range_of(s_upto, n, x);
-        if (at0 + x < a.free_cap)
-          a.free_pages[at0 + x] = a.table[(int64_t)(c0 + i) * a.table_stride + s_have[i] + x - (s_upto[i] - s_need[i])];
+  const bool once = a.num_reqs <= CHUNK;          // the one chunk's sums are still in shared memory, its requests in q
+  const int64_t given = before.give;
+  if (given > 0) {                                // the same in every CTA
+    Sums at = {0, 0, 0};
+    for (int c0 = 0; c0 < a.num_reqs; c0 += CHUNK) {
+      const int n = min(CHUNK, a.num_reqs - c0);
+      if (!once) adv_chunk(a, c, c0, count, at, total, q);
+      const int64_t at0 = count - taken + at.give;
+      const int pages = clamp31(min((int64_t)total.give, a.free_cap - at0));
+      for (int x = rank * THREADS + tid; x < pages; x += ctas * THREADS) {
+        const int i = range_of(c.gives, 0, n, x);           // its last pages, gives[i] - x of them from here
+        a.free_pages[at0 + x] = a.table[(int64_t)(c0 + i) * a.table_stride + c.have[i] - (c.gives[i] - x)];
       }
-      at0 += total;
-      __syncthreads();
+      at = at + total;
     }
-    cluster_sync();
-  }
-  for (int c = rank; c * ADV_THREADS < a.num_reqs; c += ctas) {
-    const int r = c * ADV_THREADS + tid;
-    if (r < a.num_reqs) {
-      const int64_t old = max(a.seq_lens[r], 0);
-      // status[r] was written by this thread
-      a.seq_lens[r] = a.status[r] == HKB_REQ_OK ? (int)max(old + a.new_tokens[r], (int64_t)0) : (int)old;
-    }
+    if (!once) { if (ctas > 1) cluster_sync(); else __syncthreads(); }   // the lengths are read for the last time
   }
   if (rank == 0 && tid == 0) *a.free_count = (int)min(count - taken + given, a.free_cap);
+  for (int ch = rank; ch * CHUNK < a.num_reqs; ch += ctas)
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int r = ch * CHUNK + tid * EACH + e;
+      if (r >= a.num_reqs) continue;
+      if (!once) { q[e] = adv_request(a, r); q[e].status = a.status[r]; }      // which this thread wrote
+      a.seq_lens[r] = (int)(q[e].status == HKB_REQ_OK ? max(q[e].old + q[e].grow, (int64_t)0) : q[e].old);
+    }
 }
 
 // ---------------------------------------------------------------------------------
 // A page's summary: the least and the greatest key of every channel, over the page's tokens below the
-// sequence's length. Values of the cache's own type, so nothing is rounded. A warp takes a (page, kv head): its
-// lanes hold 16-byte chunks of a row, 32 / chunks rows at a time, and fold them with packed minima and maxima
-// that keep a NaN. Bound: bytes (the keys once, two rows a page out).
+// sequence's length. Values of the cache's own type, so nothing is rounded. A warp takes a (page, kv head) -- of
+// pages of more than 32 tokens the CTA's four warps share it, or a decode step's few large pages would each be one
+// warp's chain of trips to memory: its lanes hold 16-byte chunks of a row, 32 / chunks rows at a time, and fold them
+// with packed minima and maxima that keep a NaN. Bound: bytes (the keys once, two rows a page out).
 // ---------------------------------------------------------------------------------
-constexpr int BOUNDS_WARPS = 8;
+constexpr int BOUNDS_WARPS = 4;
 
 struct BoundsArgs {
   uint8_t* bounds;                 // strides in bytes; low row, then high row, row_bytes each
@@ -231,15 +340,16 @@ __device__ __forceinline__ uint32_t f16x2_to_e4m3x2(uint32_t h2) {   // exact fo
   return r;
 }
 
-// KIND: HKB_KV_*; CPR: 16-byte chunks a row (head_dim x element size / 16)
-template <int KIND, int CPR>
+// KIND: HKB_KV_*; CPR: 16-byte chunks a row (head_dim x element size / 16); SHARE: a CTA a (page, kv head)
+template <int KIND, int CPR, bool SHARE>
 __global__ void __launch_bounds__(BOUNDS_WARPS * 32) bounds_kernel(const BoundsArgs a) {
   constexpr bool FP8 = KIND == HKB_KV_FP8_E4M3;
   using Pr = Pair<FP8 ? HKB_KV_F16 : KIND>;       // e4m3 widens to f16 exactly
   constexpr int REGS = FP8 ? 8 : 4;               // pairs a 16-byte chunk holds
   constexpr int RPI = 32 / CPR, UNROLL = 8;
-  const int lane = threadIdx.x & 31;
-  const int64_t unit = (int64_t)blockIdx.x * BOUNDS_WARPS + (threadIdx.x >> 5);
+  constexpr int STEP = RPI * UNROLL * (SHARE ? BOUNDS_WARPS : 1);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t unit = SHARE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * BOUNDS_WARPS + warp;
   const int item = (int)(unit / a.num_kv_heads), head = (int)(unit % a.num_kv_heads);
   if (item >= a.items) return;
 
@@ -278,7 +388,8 @@ __global__ void __launch_bounds__(BOUNDS_WARPS * 32) bounds_kernel(const BoundsA
   const uint8_t* src = a.k + (int64_t)block * a.k_stride_block + (int64_t)head * a.k_stride_head + (lane % CPR) * 16;
   uint32_t low[REGS], high[REGS];
   bool any = false;
-  for (int t0 = 0; t0 < live; t0 += RPI * UNROLL) {
+  int t0 = SHARE ? warp * RPI * UNROLL : 0;
+  do {                                            // at least once: a warp without rows of its own reads the last live one
     uint4 v[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {            // a row past the last live one: the last one again
@@ -296,7 +407,8 @@ __global__ void __launch_bounds__(BOUNDS_WARPS * 32) bounds_kernel(const BoundsA
       }
     }
     any = true;
-  }
+    t0 += STEP;
+  } while (t0 < live);
 #pragma unroll
   for (int x = CPR; x < 32; x <<= 1)
 #pragma unroll
@@ -304,6 +416,21 @@ __global__ void __launch_bounds__(BOUNDS_WARPS * 32) bounds_kernel(const BoundsA
       low[i] = Pr::least(low[i], __shfl_xor_sync(0xffffffffu, low[i], x));
       high[i] = Pr::most(high[i], __shfl_xor_sync(0xffffffffu, high[i], x));
     }
+  if constexpr (SHARE) {
+    __shared__ uint32_t fold[BOUNDS_WARPS - 1][2 * REGS][CPR];
+    if (warp > 0 && lane < CPR)
+#pragma unroll
+      for (int i = 0; i < REGS; ++i) { fold[warp - 1][i][lane] = low[i]; fold[warp - 1][REGS + i][lane] = high[i]; }
+    __syncthreads();
+    if (warp > 0 || lane >= CPR) return;
+#pragma unroll
+    for (int w = 0; w < BOUNDS_WARPS - 1; ++w)
+#pragma unroll
+      for (int i = 0; i < REGS; ++i) {
+        low[i] = Pr::least(low[i], fold[w][i][lane]);
+        high[i] = Pr::most(high[i], fold[w][REGS + i][lane]);
+      }
+  }
   if (lane >= CPR) return;
   uint8_t* dst = a.bounds + (int64_t)block * a.b_stride_block + (int64_t)head * a.b_stride_head + lane * 16;
   uint32_t o[2][4];
@@ -326,10 +453,18 @@ __global__ void __launch_bounds__(BOUNDS_WARPS * 32) bounds_kernel(const BoundsA
 // is q-.low + q+.high, one product of depth 2 head_dim with the summary as it lies in memory (low, then high):
 // mma.sync.m16n8k16, sixteen pages on M, the group's heads on N, as the decode walk multiplies. A warp takes a
 // (row, kv head, range of pages) and loads its fragments straight from memory: the contraction runs over dims,
-// so lane t of a quad takes eight (fp8: sixteen) consecutive ones and the query's fragments are dealt alike.
+// so lane t of a quad takes eight (fp8: sixteen) consecutive ones and the query's fragments are dealt alike. Since a
+// lane then reads nothing that another one fetched, the copies run through a cp.async ring in which every lane has its
+// own 16-byte places: asynchronous and deep as a walk's ring, without a barrier or a swizzle.
 // Bound: bytes (a summary is 2 rows a page where the attention reads 2 rows a token).
 // ---------------------------------------------------------------------------------
-constexpr int SCORE_WARPS = 4;
+constexpr int SCORE_WARPS = 1;
+template <int D, bool FP8>
+struct ScoreRing {
+  static constexpr int TILE = 16 * 2 * D * (FP8 ? 1 : 2);                       // sixteen pages' summaries
+  static constexpr int STAGES = TILE >= 16384 ? 2 : TILE >= 8192 ? 3 : 4;
+  static constexpr int BYTES = SCORE_WARPS * STAGES * TILE;
+};
 
 struct ScoreArgs {
   float* scores;
@@ -362,17 +497,45 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32) scores_kernel(const ScoreArg
   constexpr int EPC = FP8 ? 16 : 8;            // elements of a lane's 16-byte chunk
   constexpr int STEPS = D / (4 * EPC);         // chunks a lane reads of one row of D values
   constexpr int MPC = EPC / 4;                 // mma a chunk feeds
+  constexpr int CHAINS = NT == 1 ? 4 : 2;
+  using Ring = ScoreRing<D, FP8>;
+  extern __shared__ __align__(128) uint8_t hkb_smem[];
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int head = blockIdx.y, row = blockIdx.z;
-  const int first = (blockIdx.x * SCORE_WARPS + (threadIdx.x >> 5)) * a.tiles_per_warp * 16;
-  const int last = min(first + a.tiles_per_warp * 16, a.columns);
-  if (first >= last) return;
+  const int64_t first64 = ((int64_t)blockIdx.x * SCORE_WARPS + (threadIdx.x >> 5)) * a.tiles_per_warp * 16;
+  if (first64 >= a.columns) return;
+  const int first = (int)first64, last = (int)min(first64 + (int64_t)a.tiles_per_warp * 16, (int64_t)a.columns);
+  const int* table = a.table + (int64_t)row * a.table_stride;
+  // a page id a lane, two tiles at once and the next two beside them; columns past the sequence hold any number
+  auto look_up = [&](int p0) { return p0 + lane < last ? __ldg(table + p0 + lane) : 0; };
+  int ids = look_up(first), ids_next = look_up(first + 32);       // beside the length, not behind it
   const int len = max(__ldg(a.seq_lens + row), 0);
   const int pages = (int)min(((int64_t)len + a.page - 1) / a.page, (int64_t)a.columns);
   float* out = a.scores + (int64_t)row * a.s_stride_row + (int64_t)head * a.s_stride_head;
   for (int p = max(first, pages) + lane; p < last; p += 32) out[p] = -INFINITY;
   const int end = min(last, pages);
   if (first >= end) return;
+
+  const uint8_t* base = a.bounds + (int64_t)head * a.b_stride_head + t * 16;
+  const uint32_t ring = smem_u32(hkb_smem) + (threadIdx.x >> 5) * (Ring::STAGES * Ring::TILE) + lane * 16;
+  int next = first;                            // the next tile to fetch
+  auto fetch = [&](int stage) {
+    if (next < end) {
+      const uint32_t dst = ring + stage * Ring::TILE;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {            // pages g and g + 8; an id is clamped into the pool
+        const int id = __shfl_sync(0xffffffffu, ids, ((next - first) & 16) + g + 8 * j);
+        const uint8_t* src = base + (int64_t)min(max(id, 0), a.num_blocks - 1) * a.b_stride_block;
+#pragma unroll
+        for (int x = 0; x < 2 * STEPS; ++x) cp_async16(dst + (x * 2 + j) * 512, src + x * 64);
+      }
+      next += 16;
+      if (!((next - first) & 16)) { ids = ids_next; ids_next = look_up(next + 32); }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int k = 0; k < Ring::STAGES - 1; ++k) fetch(k);
 
   // the query's fragments: head g of the column tile, the dims of this lane's chunks
   uint32_t qf[NT][STEPS][EPC / 2];
@@ -412,32 +575,25 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32) scores_kernel(const ScoreArg
     }
   }
   const float factor = a.scale * (a.k_scale ? __ldg(a.k_scale) : 1.f);
-  const int* table = a.table + (int64_t)row * a.table_stride;
-  const uint8_t* base = a.bounds + (int64_t)head * a.b_stride_head + t * 16;
 
+  int stage = 0, stage_next = Ring::STAGES - 1;
   for (int p0 = first; p0 < end; p0 += 16) {
-    const uint8_t* src[2];
+    cp_async_wait<Ring::STAGES - 2>();         // this lane's own copies: nobody else's are read
+    const uint32_t tile = ring + stage * Ring::TILE;
+    stage = stage + 1 == Ring::STAGES ? 0 : stage + 1;
+    float part[CHAINS][NT][4];                 // several chains of products, so that none waits for the one before it
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {              // a page past the last one: the last one again
-      const int id = __ldg(table + min(p0 + g + 8 * j, end - 1));
-      src[j] = base + (int64_t)min(max(id, 0), a.num_blocks - 1) * a.b_stride_block;
-    }
-    float sc[NT][4];
+    for (int c = 0; c < CHAINS; ++c)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sc[nt][i] = 0.f;
+        for (int i = 0; i < 4; ++i) part[c][nt][i] = 0.f;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {     // low bounds meet the query's negative parts, high bounds the positive
-      uint4 v[STEPS][2];
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          v[s][j] = __ldg(reinterpret_cast<const uint4*>(src[j] + half * (D * (FP8 ? 1 : 2)) + s * 64));
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
-        const uint32_t x[2][4] = {{v[s][0].x, v[s][0].y, v[s][0].z, v[s][0].w}, {v[s][1].x, v[s][1].y, v[s][1].z, v[s][1].w}};
+        const uint4 v0 = lds128(tile + ((half * STEPS + s) * 2) * 512), v1 = lds128(tile + ((half * STEPS + s) * 2 + 1) * 512);
+        const uint32_t x[2][4] = {{v0.x, v0.y, v0.z, v0.w}, {v1.x, v1.y, v1.z, v1.w}};
 #pragma unroll
         for (int m = 0; m < MPC; ++m) {
           uint32_t f[4];
@@ -452,11 +608,19 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32) scores_kernel(const ScoreArg
             uint32_t b[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) b[i] = half ? Pr::most(qf[nt][s][2 * m + i], 0u) : Pr::least(qf[nt][s][2 * m + i], 0u);
-            mma16<F16>(sc[nt], f, b);
+            mma16<F16>(part[(half * (CHAINS / 2) + m % (CHAINS / 2))][nt], f, b);
           }
         }
       }
     }
+    float sc[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sc[nt][i] = CHAINS == 4 ? (part[0][nt][i] + part[1][nt][i]) + (part[2][nt][i] + part[CHAINS - 1][nt][i]) : part[0][nt][i] + part[1][nt][i];
+    fetch(stage_next);                         // over the tile before this one
+    stage_next = stage_next + 1 == Ring::STAGES ? 0 : stage_next + 1;
     // the greatest over the group's heads: this lane holds heads 2t, 2t + 1 of pages g and g + 8
     float best[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -478,17 +642,26 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32) scores_kernel(const ScoreArg
     const int p = p0 + g + 8 * (t & 1);
     if (t < 2 && p < end) out[p] = (t ? best[1] : best[0]) * factor;
   }
+  cp_async_wait<0>();
 }
 
 // ---------------------------------------------------------------------------------
 // The budget's best pages of a (row, kv head): the first `first` and the last `last` pages always, then by score
 // downwards, ties to the lowest page; written in ascending order, -1 behind. A score becomes a 32-bit key whose
-// order is the scores' (NaN above everything but the pages that are always kept: a broken key shows in the
-// answer instead of being left out); the budget-th greatest key is found digit by digit, eight bits a pass over
-// histograms in shared memory, and one more pass writes the pages that lie above it and as many of those on it
-// as there is room for. Integers throughout, so the answer depends on no order of anything.
+// order is the scores' (NaN above everything: a broken key shows in the answer instead of being left out).
+// Integers throughout: the answer depends on no order of anything. Bound: latency.
+//
+// Narrow tables (select_warp_kernel): a warp takes a (row, kv head), its lanes hold the keys in registers, every
+// 32nd page a lane, and the border is bisected between the least and the greatest key: a step is one comparison a
+// key and one warp-wide sum, and it ends as soon as a step leaves exactly the budget above it -- ten-odd steps, no
+// barrier, no memory but the one trip for the scores.
+//
+// Wide ones (select_kernel): a CTA takes it, EACH keys a thread in registers where the table's width lets it, and the
+// border is found by digits: the keys, less the least of them and shifted up to the full width, fall into 2048 bins
+// of a histogram in shared memory (so shifted, scores that differ little still spread over the bins and their atomics
+// over the banks); the bin that the border falls into is cut into 2048 again until all of it is taken or it is one value.
 // ---------------------------------------------------------------------------------
-constexpr int SELECT_THREADS = 256;
+constexpr int SELECT_BINS = 2048, SELECT_BITS = 11;
 
 struct SelectArgs {
   int* pages;
@@ -508,67 +681,219 @@ __device__ __forceinline__ uint32_t score_key(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(SELECT_THREADS) select_kernel(const SelectArgs a) {
-  __shared__ int hist[256];
-  __shared__ int warp_sum[SELECT_THREADS / 32][2];
-  __shared__ int s_digit, s_above;
+constexpr int SELECT_WARPS = 4;
+
+template <int EACH>
+__global__ void __launch_bounds__(SELECT_WARPS * 32) select_warp_kernel(const SelectArgs a, int num_kv_heads, int64_t items) {
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * SELECT_WARPS + (threadIdx.x >> 5);
+  if (item >= items) return;
+  const int64_t row = item / num_kv_heads, head = item - row * num_kv_heads;
+  const int len = max(__ldg(a.seq_lens + row), 0);
+  int* out = a.pages + row * a.p_stride_row + head * a.p_stride_head;
+  const float* in = a.scores + row * a.s_stride_row + head * a.s_stride_head;
+  // every column's key is asked for beside the length, not behind it
+  float x[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) x[e] = e * 32 + lane < a.columns ? __ldg(in + e * 32 + lane) : 0.f;
+  const int n = (int)min(((int64_t)len + a.page - 1) / a.page, (int64_t)a.columns);
+  if (n <= a.budget) {
+    for (int i = lane; i < a.budget; i += 32) out[i] = i < n ? i : -1;
+    return;
+  }
+  const int end = n - a.last;
+  int want = a.budget - a.first - a.last;         // of the candidates, pages first .. end
+  uint32_t key[EACH], least = 0xffffffffu, most = 0u;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int p = e * 32 + lane;
+    key[e] = score_key(x[e]);
+    if (p >= a.first && p < end) { least = min(least, key[e]); most = max(most, key[e]); }
+  }
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  // The greatest `lo` that at least `want` candidates reach; `reach` of them do. Keys that no candidate can have
+  // stand for the pages always kept (above all) and those past the sequence (key 0 below all: a score's is at least 2^22).
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int p = e * 32 + lane;
+    if (p < a.first || p >= end) key[e] = p < n ? 0xffffffffu : 0u;
+  }
+  const int kept = a.first + a.last;
+  uint32_t lo = want > 0 ? least : 0xffffffffu, hi = most;     // in [lo, hi]
+  int reach = want > 0 ? end - a.first : 0;
+  while (lo < hi && reach != want) {
+    const uint32_t mid = lo + ((hi - lo) >> 1) + 1u;           // lo < mid <= hi
+    int c = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) c += key[e] >= mid;
+    c = __reduce_add_sync(0xffffffffu, c) - kept;
+    if (c >= want) { lo = mid; reach = c; } else hi = mid - 1u;
+  }
+  // Taken: keys above lo, and of those equal to it the first that there is room for.
+  const bool all = reach == want;
+  int at = 0;
+  // ties: how many of the keys equal to lo are taken
+  int ties = 0x7fffffff;
+  if (!all) {
+    int c = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) c += key[e] > lo;
+    ties = want - (__reduce_add_sync(0xffffffffu, c) - kept);
+  }
+  const unsigned below = (1u << lane) - 1u;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const bool tie = !all && key[e] == lo;
+    const unsigned t = __ballot_sync(0xffffffffu, tie);
+    const bool take = key[e] > lo || (all && key[e] == lo) || (tie && __popc(t & below) < ties);
+    const unsigned w = __ballot_sync(0xffffffffu, take);
+    if (take) out[at + __popc(w & below)] = e * 32 + lane;
+    at += __popc(w);
+    ties -= min(ties, __popc(t));
+  }
+}
+
+// Inclusive sum over the CTA's threads; `sums` is one value a warp, free to be written (a barrier behind its last read).
+template <int THREADS>
+__device__ __forceinline__ uint64_t select_scan(uint64_t v, uint64_t* sums, uint64_t& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    const uint64_t y = __shfl_up_sync(0xffffffffu, v, x);
+    if (lane >= x) v += y;
+  }
+  if (lane == 31) sums[warp] = v;
+  __syncthreads();
+  uint64_t w = lane < THREADS / 32 ? sums[lane] : 0;
+  const uint64_t own = w;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    const uint64_t y = __shfl_up_sync(0xffffffffu, w, x);
+    if (lane >= x) w += y;
+  }
+  total = __shfl_sync(0xffffffffu, w, 31);
+  return v + __shfl_sync(0xffffffffu, w - own, warp);
+}
+
+// RESIDENT: THREADS x EACH covers the row; otherwise the keys are read again for every pass, THREADS x EACH at a time.
+template <int THREADS, int EACH, bool RESIDENT>
+__global__ void __launch_bounds__(THREADS) select_kernel(const SelectArgs a) {
+  __shared__ int hist[SELECT_BINS];
+  __shared__ uint32_t ends[2][THREADS / 32];
+  __shared__ uint64_t sums[2][THREADS / 32];
+  __shared__ int s_bin, s_above, s_in;
+  constexpr int MINE = SELECT_BINS / THREADS, SPAN = THREADS * EACH;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int head = blockIdx.y, row = blockIdx.x;
   const int len = max(__ldg(a.seq_lens + row), 0);
   const int n = (int)min(((int64_t)len + a.page - 1) / a.page, (int64_t)a.columns);
   int* out = a.pages + (int64_t)row * a.p_stride_row + (int64_t)head * a.p_stride_head;
-  const float* in = a.scores + (int64_t)row * a.s_stride_row + (int64_t)head * a.s_stride_head;
+  const float* in = a.scores + (int64_t)row * a.s_stride_row + (int64_t)head * a.s_stride_head + a.first;
   if (n <= a.budget) {
-    for (int i = tid; i < a.budget; i += SELECT_THREADS) out[i] = i < n ? i : -1;
+    for (int i = tid; i < a.budget; i += THREADS) out[i] = i < n ? i : -1;
     return;
   }
-  auto key = [&](int p) -> uint32_t {
-    return p < a.first || p >= n - a.last ? 0xffffffffu : score_key(__ldg(in + p));
+  // the pages that are always kept, then the candidates between them
+  for (int i = tid; i < a.first; i += THREADS) out[i] = i;
+  for (int i = tid; i < a.last; i += THREADS) out[a.budget - a.last + i] = n - a.last + i;
+  const int m = n - a.first - a.last;
+  int want = a.budget - a.first - a.last;         // of the candidates not yet decided
+  if (want == 0) return;
+  out += a.first;
+
+  uint32_t key[EACH];
+  auto load = [&](int p0) {                       // consecutive pages a thread
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int p = p0 + tid * EACH + e;
+      key[e] = p < m ? score_key(__ldg(in + p)) : 0u;
+    }
   };
-  uint32_t prefix = 0;      // the digits found so far
-  int want = a.budget;      // how many of the keys that begin with them are to be taken
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    hist[tid] = 0;
-    __syncthreads();
-    for (int p = tid; p < n; p += SELECT_THREADS) {
-      const uint32_t k = key(p);
-      if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
-    }
-    __syncthreads();
-    // the digit whose keys, with all greater ones, first reach `want`: a scan from the top
-    const int mine = hist[255 - tid];
-    int incl = mine;
 #pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, incl, x);
-      if (lane >= x) incl += y;
-    }
-    if (lane == 31) warp_sum[warp][0] = incl;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) incl += warp_sum[w][0];
-    if (incl >= want && incl - mine < want) { s_digit = 255 - tid; s_above = incl - mine; }
-    __syncthreads();
-    prefix = prefix << 8 | (uint32_t)s_digit;
-    want -= s_above;
-    __syncthreads();
+  for (int i = 0; i < MINE; ++i) hist[tid * MINE + i] = 0;
+  uint32_t least = 0xffffffffu, most = 0u;
+  for (int p0 = 0; p0 < m; p0 += SPAN) {
+    load(p0);
+#pragma unroll
+    for (int e = 0; e < EACH; ++e)
+      if (p0 + tid * EACH + e < m) { least = min(least, key[e]); most = max(most, key[e]); }
   }
-  int taken = 0, ties = 0;  // so far, over the whole CTA
-  for (int p0 = 0; p0 < n; p0 += SELECT_THREADS) {
-    const int p = p0 + tid;
-    const uint32_t k = p < n ? key(p) : 0u;
-    const bool tie = p < n && k == prefix, above = p < n && k > prefix;
-    const unsigned mt = __ballot_sync(0xffffffffu, tie), ma = __ballot_sync(0xffffffffu, above);
-    if (lane == 0) { warp_sum[warp][0] = __popc(ma); warp_sum[warp][1] = __popc(mt); }
-    __syncthreads();
-    const unsigned below = (1u << lane) - 1;
-    int at = taken + __popc(ma & below), tie_at = ties + __popc(mt & below);
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) { ends[0][warp] = least; ends[1][warp] = most; }
+  __syncthreads();
+  least = __reduce_min_sync(0xffffffffu, lane < THREADS / 32 ? ends[0][lane] : 0xffffffffu);
+  most = __reduce_max_sync(0xffffffffu, lane < THREADS / 32 ? ends[1][lane] : 0u);
+
+  // Keys from `base` on that are below base + 2^(32 - shift) are undecided; all greater ones are taken.
+  uint32_t base = least;
+  int shift = __clz(most - least), which = 0;     // 32: they are all one value
+  bool whole = false;                             // all undecided keys are taken
+  while (shift < 32) {
+    for (int p0 = 0; p0 < m; p0 += SPAN) {
+      if (!RESIDENT) load(p0);
 #pragma unroll
-    for (int w = 0; w < SELECT_THREADS / 32; ++w) {
-      if (w < warp) { at += warp_sum[w][0]; tie_at += warp_sum[w][1]; }
-      taken += warp_sum[w][0]; ties += warp_sum[w][1];
+      for (int e = 0; e < EACH; ++e) {
+        const uint32_t x = key[e] - base;         // a key below base wraps to a great x
+        if (p0 + tid * EACH + e < m && key[e] >= base && (x >> (31 - shift)) <= 1u)
+          atomicAdd(&hist[(x << shift) >> (32 - SELECT_BITS)], 1);
+      }
     }
-    if (above || (tie && tie_at < want)) out[at + min(tie_at, want)] = p;
     __syncthreads();
+    // the bin in which the keys, counted from the top, reach `want`; the bins are cleared for the next pass
+    int bins[MINE], mine = 0;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      bins[i] = hist[SELECT_BINS - 1 - tid * MINE - i];
+      hist[SELECT_BINS - 1 - tid * MINE - i] = 0;
+      mine += bins[i];
+    }
+    uint64_t total;
+    int above = (int)select_scan<THREADS>((uint64_t)mine, sums[which], total) - mine;
+    which ^= 1;
+    if (above < want && above + mine >= want) {   // one thread
+      int i = 0;
+#pragma unroll
+      for (int j = 0; j < MINE - 1; ++j)
+        if (i == j && above + bins[j] < want) { above += bins[j]; ++i; }
+      int in_bin = 0;
+#pragma unroll
+      for (int j = 0; j < MINE; ++j)
+        if (i == j) in_bin = bins[j];
+      s_bin = SELECT_BINS - 1 - tid * MINE - i; s_above = above; s_in = in_bin;
+    }
+    __syncthreads();
+    want -= s_above;
+    base += ((uint32_t)s_bin << (32 - SELECT_BITS)) >> shift;
+    if (s_in == want) { whole = true; break; }
+    shift += SELECT_BITS;                         // 32 and more: the bin is one value
+  }
+  // Taken: keys above `base`; of those equal to it the first `want` -- or all from it on, where `whole`.
+  uint64_t done = 0;                              // keys above in the upper half, ties in the lower
+  for (int p0 = 0; p0 < m; p0 += SPAN) {
+    if (!RESIDENT) load(p0);
+    uint64_t mine = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      if (p0 + tid * EACH + e >= m) continue;
+      if (whole ? key[e] >= base : key[e] > base) mine += 1ull << 32;
+      else if (!whole && key[e] == base) mine += 1;
+    }
+    uint64_t total;
+    const uint64_t incl = done + select_scan<THREADS>(mine, sums[which], total);
+    which ^= 1;
+    done += total;
+    int at = (int)((incl - mine) >> 32), ties = (int)(uint32_t)(incl - mine);
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int p = p0 + tid * EACH + e;
+      if (p >= m) continue;
+      const bool tie = !whole && key[e] == base;
+      if ((whole ? key[e] >= base : key[e] > base) || (tie && ties < want)) out[at + min(ties, want)] = a.first + p;
+      if (tie) ++ties;
+      else if (whole ? key[e] >= base : key[e] > base) ++at;
+    }
   }
 }
 
@@ -580,6 +905,27 @@ static int launched(F&& launch) {
   return HKB_OK;
 }
 
+// More than 48 KB of dynamic shared memory, or a cluster past the portable size, is asked for once a device.
+template <class K>
+static cudaError_t arm(K kernel, cudaFuncAttribute attribute, int value, bool (&armed)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev >= 0 && dev < 64 && !armed[dev]) {
+    e = cudaFuncSetAttribute(kernel, attribute, value);
+    if (e == cudaSuccess) armed[dev] = true;
+  }
+  if (e != cudaSuccess) { (void)cudaGetLastError(); hkb_tls_cuda_error = (int)e; }
+  return e;
+}
+
+template <int KIND, int D, int NT>
+static int launch_scores(const ScoreArgs& a, dim3 grid, cudaStream_t st) {
+  static bool armed[64] = {};
+  constexpr int smem = ScoreRing<D, KIND == HKB_KV_FP8_E4M3>::BYTES;
+  if (arm(scores_kernel<KIND, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem, armed) != cudaSuccess) return HKB_ERR_CUDA;
+  return launched([&] { scores_kernel<KIND, D, NT><<<grid, SCORE_WARPS * 32, smem, st>>>(a); });
+}
+
 }  // namespace hkb
 
 extern "C" int hkb_advance_tables(int32_t* block_table, int64_t table_stride, int max_pages, int32_t* seq_lens,
@@ -587,7 +933,8 @@ extern "C" int hkb_advance_tables(int32_t* block_table, int64_t table_stride, in
                                   int64_t free_capacity, int32_t* free_count, int64_t* slot_mapping, int64_t* positions,
                                   int64_t num_rows, int32_t* q_start, int32_t* status, void* stream) {
   using namespace hkb;
-  if (num_reqs < 0 || max_pages < 0 || free_capacity < 0 || num_rows < 0 || free_capacity > 0x7fffffff) return HKB_ERR_SIZE;
+  if (num_reqs < 0 || max_pages < 0 || free_capacity < 0 || num_rows < 0 ||
+      free_capacity > 0x7fffffff || num_rows > 0x40000000 || num_reqs > 0x40000000) return HKB_ERR_SIZE;
   if (block_size <= 0) return HKB_ERR_BLOCK_SIZE;
   if (!free_count || !q_start) return HKB_ERR_NULL;
   if (num_reqs > 0 && (!seq_lens || !new_tokens || !status)) return HKB_ERR_NULL;
@@ -598,11 +945,20 @@ extern "C" int hkb_advance_tables(int32_t* block_table, int64_t table_stride, in
   AdvanceArgs a;
   a.table = block_table; a.table_stride = table_stride; a.max_pages = max_pages;
   a.seq_lens = seq_lens; a.new_tokens = new_tokens; a.num_reqs = num_reqs; a.page = block_size;
+  int l = 0;
+  while (l < 31 && (1u << l) < (uint32_t)block_size) ++l;
+  a.page_magic = l ? (uint32_t)((1ull << (31 + l)) / (uint32_t)block_size + 1) : 0;
+  a.page_shift = l ? l - 1 : 0;
   a.free_pages = free_pages; a.free_count = free_count; a.free_cap = free_capacity;
   a.slots = slot_mapping; a.positions = positions; a.tokens = num_rows;
   a.q_start = q_start; a.status = status;
-  const int ctas = num_rows > 4096 ? 8 : 1;
-  return launch_cluster((const void*)advance_kernel, dim3(ctas), ADV_THREADS, ctas, 0, &a, (cudaStream_t)stream);
+  if (num_rows > 4096 || num_reqs > 512) {
+    auto kernel = advance_kernel<32, 2>;
+    static bool armed[64] = {};
+    if (arm(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1, armed) != cudaSuccess) return HKB_ERR_CUDA;
+    return launch_cluster((const void*)kernel, dim3(16), 1024, 16, 0, &a, (cudaStream_t)stream);
+  }
+  return launch_cluster((const void*)advance_kernel<8, 2>, dim3(1), 256, 1, 0, &a, (cudaStream_t)stream);
 }
 
 extern "C" int hkb_page_bounds(void* bounds, int64_t bounds_stride_block, int64_t bounds_stride_head, int64_t bounds_blocks,
@@ -620,7 +976,8 @@ extern "C" int hkb_page_bounds(void* bounds, int64_t bounds_stride_block, int64_
   if ((kc.stride_block | kc.stride_token | kc.stride_head | bounds_stride_block | bounds_stride_head) * es % 16) return HKB_ERR_STRIDE;
   if (((uintptr_t)kc.ptr | (uintptr_t)bounds) % 16) return HKB_ERR_ALIGN;
   const int64_t items = q_start ? num_tokens / block_size + 2 * (int64_t)num_seqs : num_seqs;
-  const int64_t ctas = (items * num_kv_heads + BOUNDS_WARPS - 1) / BOUNDS_WARPS;
+  const bool share = block_size > 32;
+  const int64_t per_cta = share ? 1 : BOUNDS_WARPS, ctas = (items * num_kv_heads + per_cta - 1) / per_cta;
   if (items > 0x3fffffff || ctas > 0x7fffffff) return HKB_ERR_SIZE;
   BoundsArgs a;
   a.bounds = (uint8_t*)bounds; a.b_stride_block = bounds_stride_block * es; a.b_stride_head = bounds_stride_head * es;
@@ -634,7 +991,10 @@ extern "C" int hkb_page_bounds(void* bounds, int64_t bounds_stride_block, int64_
   cudaStream_t st = (cudaStream_t)stream;
   return launched([&] {
 #define HKB_BOUNDS(KIND, CPR_) \
-  if (kv_dtype == KIND && head_dim * es == CPR_ * 16) bounds_kernel<KIND, CPR_><<<(unsigned)ctas, BOUNDS_WARPS * 32, 0, st>>>(a);
+  if (kv_dtype == KIND && head_dim * es == CPR_ * 16) { \
+    if (share) bounds_kernel<KIND, CPR_, true><<<(unsigned)ctas, BOUNDS_WARPS * 32, 0, st>>>(a); \
+    else bounds_kernel<KIND, CPR_, false><<<(unsigned)ctas, BOUNDS_WARPS * 32, 0, st>>>(a); \
+  }
     HKB_BOUNDS(HKB_KV_BF16, 8) HKB_BOUNDS(HKB_KV_BF16, 16) HKB_BOUNDS(HKB_KV_BF16, 32)
     HKB_BOUNDS(HKB_KV_F16, 8) HKB_BOUNDS(HKB_KV_F16, 16) HKB_BOUNDS(HKB_KV_F16, 32)
     HKB_BOUNDS(HKB_KV_FP8_E4M3, 4) HKB_BOUNDS(HKB_KV_FP8_E4M3, 8) HKB_BOUNDS(HKB_KV_FP8_E4M3, 16)
@@ -669,23 +1029,24 @@ extern "C" int hkb_page_scores(float* scores, int64_t scores_stride_row, int64_t
   a.num_blocks = bounds_blocks > 0x7fffffff ? 0x7fffffff : (int)bounds_blocks;
   a.table = block_table; a.table_stride = table_stride; a.seq_lens = seq_lens;
   a.page = block_size; a.group = num_q_heads / num_kv_heads; a.scale = scale; a.k_scale = fp8 ? k_scale : nullptr;
-  a.tiles_per_warp = 2;
   const int64_t tiles = ((int64_t)num_columns + 15) / 16;
+  // as many warps as the machine holds at once, eight an SM, each a CTA of its own
+  int sms = hkb_sm_count(-1);
+  if (sms <= 0) sms = 148;
+  const int64_t room = (int64_t)sms * 8, per = (tiles * num_rows * num_kv_heads + room - 1) / room;
+  a.tiles_per_warp = (int)(per < tiles ? per : tiles);
   const int64_t warps = (tiles + a.tiles_per_warp - 1) / a.tiles_per_warp;
   const dim3 grid((unsigned)((warps + SCORE_WARPS - 1) / SCORE_WARPS), num_kv_heads, num_rows);
   cudaStream_t st = (cudaStream_t)stream;
   const int nt = a.group > 8 ? 2 : 1;
-  return launched([&] {
 #define HKB_SCORES(KIND, D_) \
-  if (kv_dtype == KIND && head_dim == D_) { \
-    if (nt == 1) scores_kernel<KIND, D_, 1><<<grid, SCORE_WARPS * 32, 0, st>>>(a); \
-    else scores_kernel<KIND, D_, 2><<<grid, SCORE_WARPS * 32, 0, st>>>(a); \
-  }
-    HKB_SCORES(HKB_KV_BF16, 64) HKB_SCORES(HKB_KV_BF16, 128) HKB_SCORES(HKB_KV_BF16, 256)
-    HKB_SCORES(HKB_KV_F16, 64) HKB_SCORES(HKB_KV_F16, 128) HKB_SCORES(HKB_KV_F16, 256)
-    HKB_SCORES(HKB_KV_FP8_E4M3, 64) HKB_SCORES(HKB_KV_FP8_E4M3, 128) HKB_SCORES(HKB_KV_FP8_E4M3, 256)
+  if (kv_dtype == KIND && head_dim == D_) \
+    return nt == 1 ? launch_scores<KIND, D_, 1>(a, grid, st) : launch_scores<KIND, D_, 2>(a, grid, st);
+  HKB_SCORES(HKB_KV_BF16, 64) HKB_SCORES(HKB_KV_BF16, 128) HKB_SCORES(HKB_KV_BF16, 256)
+  HKB_SCORES(HKB_KV_F16, 64) HKB_SCORES(HKB_KV_F16, 128) HKB_SCORES(HKB_KV_F16, 256)
+  HKB_SCORES(HKB_KV_FP8_E4M3, 64) HKB_SCORES(HKB_KV_FP8_E4M3, 128) HKB_SCORES(HKB_KV_FP8_E4M3, 256)
 #undef HKB_SCORES
-  });
+  return HKB_ERR_UNSUPPORTED;
 }
 
 extern "C" int hkb_select_pages(int32_t* pages, int64_t pages_stride_row, int64_t pages_stride_head, int budget,
@@ -703,5 +1064,17 @@ extern "C" int hkb_select_pages(int32_t* pages, int64_t pages_stride_row, int64_
   a.pages = pages; a.p_stride_row = pages_stride_row; a.p_stride_head = pages_stride_head; a.budget = budget;
   a.scores = scores; a.s_stride_row = scores_stride_row; a.s_stride_head = scores_stride_head; a.columns = num_columns;
   a.seq_lens = seq_lens; a.page = block_size; a.first = first; a.last = last;
-  return launched([&] { select_kernel<<<dim3(num_rows, num_kv_heads), SELECT_THREADS, 0, (cudaStream_t)stream>>>(a); });
+  const dim3 grid(num_rows, num_kv_heads);
+  cudaStream_t st = (cudaStream_t)stream;
+  return launched([&] {
+    const int64_t items = (int64_t)num_rows * num_kv_heads;
+    const unsigned ctas = (unsigned)((items + SELECT_WARPS - 1) / SELECT_WARPS);
+    if (num_columns <= 256) select_warp_kernel<8><<<ctas, SELECT_WARPS * 32, 0, st>>>(a, num_kv_heads, items);
+    else if (num_columns <= 512) select_warp_kernel<16><<<ctas, SELECT_WARPS * 32, 0, st>>>(a, num_kv_heads, items);
+    else if (num_columns <= 1024) select_warp_kernel<32><<<ctas, SELECT_WARPS * 32, 0, st>>>(a, num_kv_heads, items);
+    else if (num_columns <= 2048) select_kernel<256, 8, true><<<grid, 256, 0, st>>>(a);
+    else if (num_columns <= 8192) select_kernel<1024, 8, true><<<grid, 1024, 0, st>>>(a);
+    else if (num_columns <= 16384) select_kernel<1024, 16, true><<<grid, 1024, 0, st>>>(a);
+    else select_kernel<1024, 16, false><<<grid, 1024, 0, st>>>(a);
+  });
 }

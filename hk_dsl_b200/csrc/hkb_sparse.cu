@@ -56,10 +56,9 @@ __global__ void __launch_bounds__(WARPS * 32) sparse_kernel(const SparseArgs a) 
     const int e = (int)x / tpp, sub = (int)x - e * tpp;
     const int p = __ldg(list + e);
     if (p < 0 || p >= a.d.max_pages) return;
+    id = __ldg(table + p);                            // asked for beside the length, not behind it
     const int64_t t0 = (int64_t)p * a.d.block_size + sub * TILE_TOKENS;
-    if (t0 >= seq_len) return;
-    tok = (int)t0;
-    id = __ldg(table + p);
+    if (t0 < seq_len) tok = (int)t0;
   };
   int next_item = 64, id, tok, id_n, tok_n;
   look_up(0, id, tok);
@@ -115,28 +114,56 @@ __global__ void __launch_bounds__(WARPS * 32) sparse_kernel(const SparseArgs a) 
       const int h = nt * 8 + 2 * (lane & 3) + c;
       if ((lane >> 2) == 0 && h < nh && (bad & (0x11111111u << (lane & 3)))) part[HEADS * D + h] = NAN;
     }
-  cluster_sync();
+  if (ctas > 1) cluster_sync(); else __syncthreads();
 
-  // Fold: a quad of output columns a thread, over all workers' partials.
+  // Fold: this CTA's slice of the outputs, four columns a quad; `ways` lanes share a quad and take every ways-th
+  // worker, four of them requested at once (lse and values together: one trip to the peers for up to 4 ways workers).
   const uint32_t mem = smem_u32(hkb_smem);
-  const int quads = nh * (D / 4), share = (quads + ctas - 1) / ctas;
-  const int x1 = min(quads, (rank + 1) * share);
-  for (int x = rank * share + threadIdx.x; x < x1; x += WARPS * 32) {
-    const int h = x / (D / 4), c = x % (D / 4);
-    float mx = -INFINITY;
-    for (int r = 0; r < ctas; ++r)
-      for (int w = 0; w < WARPS; ++w) mx = fmaxf(mx, peer_f1(peer_smem(mem + w * P::RING_SMEM + (HEADS * D + h) * 4, r)));
-    float den = 0.f;
+  const int quads = nh * (D / 4), share = (quads + ctas - 1) / ctas, x0 = rank * share, slice = min(quads, x0 + share) - x0;
+  int ways = 1;
+  while (ways < 32 && ways * 4 < workers && ways * 2 * share <= WARPS * 32) ways *= 2;
+  const int sub = threadIdx.x & (ways - 1), rows_at_once = WARPS * 32 / ways;
+  for (int y = 0; y < slice; y += rows_at_once) {       // uniform over the CTA
+    const int x = x0 + y + threadIdx.x / ways;
+    const bool mine = x < x0 + slice;
+    const int h = mine ? x / (D / 4) : 0, c = x % (D / 4);
+    float mx = -INFINITY, den = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int r = 0; r < ctas; ++r)
-      for (int w = 0; w < WARPS; ++w) {
-        const uint32_t at = peer_smem(mem + w * P::RING_SMEM, r);
-        const float lse = peer_f1(at + (HEADS * D + h) * 4);
-        const float wt = lse == -INFINITY ? 0.f : fast_exp2((lse - mx) * LOG2E);
-        const float4 v = peer_f4(at + (h * D + c * 4) * 4);
-        den += wt;
-        acc.x = fmaf(wt, v.x, acc.x); acc.y = fmaf(wt, v.y, acc.y); acc.z = fmaf(wt, v.z, acc.z); acc.w = fmaf(wt, v.w, acc.w);
+    for (int j0 = sub; j0 < workers; j0 += 4 * ways) {
+      float lse[4];
+      float4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = j0 + u * ways;
+        lse[u] = -INFINITY; v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (mine && j < workers) {
+          const uint32_t at = peer_smem(mem + (j % WARPS) * P::RING_SMEM, j / WARPS);
+          lse[u] = peer_f1(at + (HEADS * D + h) * 4);
+          v[u] = peer_f4(at + (h * D + c * 4) * 4);
+        }
       }
+      const float top = fmaxf(mx, fmaxf(fmaxf(lse[0], lse[1]), fmaxf(lse[2], lse[3])));
+      const float ref = top == -INFINITY ? 0.f : top;
+      const float keep = fast_exp2((mx - ref) * LOG2E);  // 0 while nothing has been seen
+      den *= keep; acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+      mx = top;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float wt = fast_exp2((lse[u] - ref) * LOG2E);
+        den += wt;
+        acc.x = fmaf(wt, v[u].x, acc.x); acc.y = fmaf(wt, v[u].y, acc.y); acc.z = fmaf(wt, v[u].z, acc.z); acc.w = fmaf(wt, v[u].w, acc.w);
+      }
+    }
+    for (int o = 1; o < ways; o <<= 1) {
+      const float top = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float keep = fast_exp2((mx - (top == -INFINITY ? 0.f : top)) * LOG2E);
+      mx = top;
+      den *= keep; acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+      den += __shfl_xor_sync(0xffffffffu, den, o);
+      acc.x += __shfl_xor_sync(0xffffffffu, acc.x, o); acc.y += __shfl_xor_sync(0xffffffffu, acc.y, o);
+      acc.z += __shfl_xor_sync(0xffffffffu, acc.z, o); acc.w += __shfl_xor_sync(0xffffffffu, acc.w, o);
+    }
+    if (!mine || sub) continue;
     const float inv = den == 0.f ? 0.f : 1.f / den;
     uint2 o;
     o.x = pack16x2<F16>(acc.x * inv, acc.y * inv);
@@ -145,7 +172,7 @@ __global__ void __launch_bounds__(WARPS * 32) sparse_kernel(const SparseArgs a) 
     if (a.out_lse && c == 0)
       a.out_lse[(int64_t)row * a.d.num_q_heads + hq0 + h] = den == 0.f ? -INFINITY : mx + logf(den);
   }
-  cluster_sync();                // no CTA leaves while a peer reads its memory
+  if (ctas > 1) cluster_sync();  // no CTA leaves while a peer reads its memory
 }
 
 template <class P, int WARPS, bool F16>

@@ -26,17 +26,37 @@ from typing import Optional
 import torch
 
 from ..runtime import lib as _lib
-from .paged import ACT_DTYPES, _FP8_DTYPES, _cache_t, _need_cuda, _scale_ptr, _stream, kv_dtype_code
+from .paged import _FP8_DTYPES, _need_cuda, _scale_ptr, kv_dtype_code
 
 #: `status` of `advance_tables`
 REQ_OK, REQ_NO_PAGES, REQ_TABLE_FULL, REQ_NO_ROWS = 0, 1, 2, 3
 
 _WHO = "hk.ops.paged_sparse"
+_I32, _I64, _F32, _BF16, _F16 = torch.int32, torch.int64, torch.float32, torch.bfloat16, torch.float16
+
+# A decode step makes a handful of these calls a layer, each a few microseconds on the GPU, so what the host spends on a
+# call counts. Tensors' sizes and strides are read once a call, devices by number, and the stream's handle is taken
+# straight from torch's binding where it has one (2.3 us a call through torch.cuda.current_stream, 0.1 us so).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _int32(name: str, t: torch.Tensor, dim: int, dtype=torch.int32) -> None:
+def _on(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """The current stream's handle, where every tensor is on the current CUDA device; else what `_need_cuda` raises."""
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            break
+    else:
+        if dev >= 0 and dev == torch.cuda.current_device():
+            return _raw_stream(dev)
+    _need_cuda(first, *others)
+    raise RuntimeError(f"{_WHO}: tensors on different devices")
+
+
+def _index(name: str, t: torch.Tensor, dim: int, dtype=_I32) -> None:
     """An index tensor: `dim` axes, the last one contiguous."""
-    if t.dim() != dim or t.dtype != dtype or (t.shape[-1] > 1 and t.stride(-1) != 1):
+    if t.dtype is not dtype or t.dim() != dim or not (t.is_contiguous() or t.shape[-1] <= 1 or t.stride(-1) == 1):
         raise TypeError(f"{_WHO}: {name} is {tuple(t.shape)} {t.dtype} strides {tuple(t.stride())}; "
                         f"{dim}-dimensional {dtype} with a contiguous last axis needed")
 
@@ -47,12 +67,15 @@ def _page_size(block_size: int) -> int:
     return int(block_size)
 
 
-def _tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, rows: int) -> None:
-    _int32("block_tables", block_tables, 2)
-    _int32("seq_lens", seq_lens, 1)
-    if block_tables.shape[0] < rows or seq_lens.shape[0] < rows:
+def _tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, rows: int) -> int:
+    """The checked table's width."""
+    _index("block_tables", block_tables, 2)
+    _index("seq_lens", seq_lens, 1)
+    have, width = block_tables.shape
+    if have < rows or seq_lens.shape[0] < rows:
         raise ValueError(f"{_WHO}: block_tables {tuple(block_tables.shape)} and seq_lens {tuple(seq_lens.shape)} "
                          f"for {rows} rows")
+    return width
 
 
 def page_bounds(key_cache: torch.Tensor) -> torch.Tensor:
@@ -76,44 +99,69 @@ def advance_tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, new_token
     one (`reshape_and_cache` skips them, so a captured step may have spare rows); `status` (requests,) int32. A request
     with `REQ_NO_PAGES` (too few free pages; once one is short, so is every later one that needs any), `REQ_TABLE_FULL`
     or `REQ_NO_ROWS` keeps its length, gets no page, and its rows get slot -1. A page belongs to one request."""
-    n = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
-    _int32("block_tables", block_tables, 2)
-    for name, t in (("seq_lens", seq_lens), ("new_tokens", new_tokens), ("free_pages", free_pages),
-                    ("free_count", free_count), ("query_start_loc", query_start_loc), ("status", status)):
-        _int32(name, t, 1)
-    _int32("slot_mapping", slot_mapping, 1, torch.int64)
-    _int32("positions", positions, 1, torch.int64)
-    if block_tables.shape[0] < n or new_tokens.shape[0] < n or status.shape[0] < n or query_start_loc.shape[0] < n + 1:
+    _index("block_tables", block_tables, 2)
+    _index("seq_lens", seq_lens, 1)
+    _index("new_tokens", new_tokens, 1)
+    _index("free_pages", free_pages, 1)
+    _index("free_count", free_count, 1)
+    _index("query_start_loc", query_start_loc, 1)
+    _index("status", status, 1)
+    _index("slot_mapping", slot_mapping, 1, _I64)
+    _index("positions", positions, 1, _I64)
+    n, = seq_lens.shape
+    have, width = block_tables.shape
+    stride = block_tables.stride(0)
+    rows, = slot_mapping.shape
+    if have < n or new_tokens.shape[0] < n or status.shape[0] < n or query_start_loc.shape[0] < n + 1:
         raise ValueError(f"{_WHO}: {n} requests (seq_lens) with block_tables {tuple(block_tables.shape)}, new_tokens "
                          f"{tuple(new_tokens.shape)}, status {tuple(status.shape)}, query_start_loc "
                          f"{tuple(query_start_loc.shape)} ({n + 1} needed)")
-    if free_count.numel() < 1 or positions.shape[0] != slot_mapping.shape[0]:
+    if free_count.shape[0] < 1 or positions.shape[0] != rows:
         raise ValueError(f"{_WHO}: free_count holds {free_count.numel()} numbers (1 needed); slot_mapping "
                          f"{tuple(slot_mapping.shape)} and positions {tuple(positions.shape)} must be alike")
-    if n > 1 and block_tables.stride(0) < block_tables.shape[1]:
+    if n > 1 and stride < width:
         raise ValueError(f"{_WHO}: block_tables' rows overlap (strides {tuple(block_tables.stride())}); it is written")
-    _need_cuda(block_tables, seq_lens, new_tokens, free_pages, free_count, slot_mapping, positions, query_start_loc, status)
-    _lib.check("hkb_advance_tables", _lib.load().hkb_advance_tables(
-        block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(),
-        new_tokens.data_ptr(), n, _page_size(block_size), free_pages.data_ptr(), free_pages.shape[0],
-        free_count.data_ptr(), slot_mapping.data_ptr(), positions.data_ptr(), slot_mapping.shape[0],
-        query_start_loc.data_ptr(), status.data_ptr(), _stream(seq_lens)))
+    page = _page_size(block_size)
+    stream = _on(seq_lens, block_tables, new_tokens, free_pages, free_count, slot_mapping, positions, query_start_loc, status)
+    rc = _lib.load().hkb_advance_tables(
+        block_tables.data_ptr(), stride, width, seq_lens.data_ptr(), new_tokens.data_ptr(), n, page,
+        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), slot_mapping.data_ptr(), positions.data_ptr(),
+        rows, query_start_loc.data_ptr(), status.data_ptr(), stream)
+    if rc:
+        _lib.check("hkb_advance_tables", rc)
 
 
 def _kind(cache: torch.Tensor) -> int:
-    code = {torch.bfloat16: _lib.KV_BF16, torch.float16: _lib.KV_F16}.get(cache.dtype)
-    if code is None:
-        if cache.dtype not in _FP8_DTYPES:
-            raise TypeError(f"{_WHO}: a key cache of {cache.dtype} (bfloat16, float16 and float8_e4m3fn, or uint8 for "
-                            f"the latter's bytes, are implemented)")
-        code = _lib.KV_FP8_E4M3
-    return code
+    dtype = cache.dtype
+    if dtype is _BF16:
+        return _lib.KV_BF16
+    if dtype is _F16:
+        return _lib.KV_F16
+    if dtype not in _FP8_DTYPES:
+        raise TypeError(f"{_WHO}: a key cache of {dtype} (bfloat16, float16 and float8_e4m3fn, or uint8 for the latter's "
+                        f"bytes, are implemented)")
+    return _lib.KV_FP8_E4M3
 
 
-def _check_bounds(bounds: torch.Tensor) -> None:
-    if bounds.dim() != 4 or bounds.shape[2] != 2 or bounds.stride(3) != 1 or bounds.stride(2) != bounds.shape[3]:
-        raise ValueError(f"{_WHO}: bounds is {tuple(bounds.shape)} strides {tuple(bounds.stride())}; "
+def _cache_strides(key_cache: torch.Tensor, value_cache: Optional[torch.Tensor] = None):
+    """A cache's shape and strides (the value cache's too), checked: head_dim contiguous."""
+    shape, ks = key_cache.shape, key_cache.stride()
+    vs = value_cache.stride() if value_cache is not None else ks
+    if len(shape) != 4 or ks[3] != 1 or vs[-1] != 1 or (value_cache is not None and (
+            value_cache.shape != shape or value_cache.dtype is not key_cache.dtype)):
+        other = "" if value_cache is None else \
+            f" / value_cache {tuple(value_cache.shape)} {value_cache.dtype} strides {tuple(vs)}"
+        raise ValueError(f"{_WHO}: key_cache {tuple(shape)} {key_cache.dtype} strides {tuple(ks)}{other}; "
+                         f"(blocks, block_size, kv_heads, head_dim) views of one dtype with head_dim contiguous needed")
+    return shape, ks, vs
+
+
+def _bounds_strides(bounds: torch.Tensor):
+    shape, strides = bounds.shape, bounds.stride()
+    if len(shape) != 4 or shape[2] != 2 or strides[3] != 1 or strides[2] != shape[3]:
+        raise ValueError(f"{_WHO}: bounds is {tuple(shape)} strides {tuple(strides)}; "
                          f"(blocks, kv_heads, 2, head_dim) with the last two axes contiguous needed (page_bounds)")
+    return shape, strides
 
 
 def update_page_bounds(bounds: torch.Tensor, key_cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
@@ -126,29 +174,29 @@ def update_page_bounds(bounds: torch.Tensor, key_cache: torch.Tensor, block_tabl
     host number, is at least its last entry (the step's rows). A sequence without new tokens has its last page summarised
     again: it holds fewer tokens if the sequence was shortened. `bounds` is of the cache's type: nothing is rounded. Pages
     are read from the cache as it is, so a call may be repeated; sequences of length 0 are left out."""
-    if key_cache.dim() != 4 or key_cache.stride(3) != 1:
-        raise ValueError(f"{_WHO}: key_cache {tuple(key_cache.shape)} strides {tuple(key_cache.stride())}; "
-                         f"(blocks, block_size, kv_heads, head_dim) with head_dim contiguous needed")
-    _check_bounds(bounds)
-    nb, page, hkv, d = key_cache.shape
+    (nb, page, hkv, d), ks, _ = _cache_strides(key_cache)
+    bshape, bs = _bounds_strides(bounds)
     code = _kind(key_cache)
-    if bounds.dtype != key_cache.dtype or bounds.shape[1] != hkv or bounds.shape[3] != d:
+    if bounds.dtype is not key_cache.dtype or bshape[1] != hkv or bshape[3] != d:
         raise ValueError(f"{_WHO}: bounds {tuple(bounds.shape)} {bounds.dtype} beside a key cache {tuple(key_cache.shape)} "
                          f"{key_cache.dtype}")
     n = seq_lens.shape[0]
-    _tables(block_tables, seq_lens, n)
+    width = _tables(block_tables, seq_lens, n)
+    starts = None
     if query_start_loc is not None:
-        _int32("query_start_loc", query_start_loc, 1)
+        _index("query_start_loc", query_start_loc, 1)
         if query_start_loc.shape[0] < n + 1:
             raise ValueError(f"{_WHO}: query_start_loc has {query_start_loc.shape[0]} entries for {n} sequences")
         if num_tokens is None or num_tokens < 0:
             raise ValueError(f"{_WHO}: query_start_loc needs num_tokens, the rows of the step (a host number), not {num_tokens}")
-    _need_cuda(bounds, key_cache, block_tables, seq_lens, query_start_loc)
-    _lib.check("hkb_page_bounds", _lib.load().hkb_page_bounds(
-        bounds.data_ptr(), bounds.stride(0), bounds.stride(1), bounds.shape[0], _cache_t(key_cache),
-        block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(),
-        query_start_loc.data_ptr() if query_start_loc is not None else None, n, num_tokens or 0, hkv, d, page, code,
-        _stream(bounds)))
+        starts = query_start_loc.data_ptr()
+    stream = _on(bounds, key_cache, block_tables, seq_lens, query_start_loc)
+    rc = _lib.load().hkb_page_bounds(
+        bounds.data_ptr(), bs[0], bs[1], bshape[0], _lib.CacheT(key_cache.data_ptr(), ks[0], ks[1], ks[2], nb),
+        block_tables.data_ptr(), block_tables.stride(0), width, seq_lens.data_ptr(), starts, n, num_tokens or 0, hkv, d,
+        page, code, stream)
+    if rc:
+        _lib.check("hkb_page_bounds", rc)
     return bounds
 
 
@@ -159,10 +207,13 @@ def _positive(scale: float) -> float:
     return scale
 
 
-def _query(name: str, t: torch.Tensor) -> None:
-    if t.dim() != 3 or t.dtype not in ACT_DTYPES or t.stride(2) != 1:
-        raise ValueError(f"{_WHO}: {name} is {tuple(t.shape)} {t.dtype} strides {tuple(t.stride())}; "
+def _query(query: torch.Tensor):
+    """The query's shape and strides, checked."""
+    shape, strides, dtype = query.shape, query.stride(), query.dtype
+    if len(shape) != 3 or strides[2] != 1 or (dtype is not _BF16 and dtype is not _F16):
+        raise ValueError(f"{_WHO}: query is {tuple(shape)} {dtype} strides {tuple(strides)}; "
                          f"(rows, q_heads, head_dim) bfloat16 or float16 with head_dim contiguous needed")
+    return shape, strides
 
 
 def page_scores(scores: torch.Tensor, query: torch.Tensor, bounds: torch.Tensor, block_tables: torch.Tensor,
@@ -173,26 +224,24 @@ def page_scores(scores: torch.Tensor, query: torch.Tensor, bounds: torch.Tensor,
     `scores` (rows, kv_heads, max_pages) fp32 gets `scale * k_scale * max_g sum_d max(q_gd low_d, q_gd high_d)`, the
     greatest over the kv head's group of query heads, and -inf for the table's columns behind the sequence.
     `query` (rows, q_heads, head_dim); `bounds` from `update_page_bounds`."""
-    _query("query", query)
-    _check_bounds(bounds)
-    rows, hq, d = query.shape
-    nb, hkv, _, bd = bounds.shape
-    width = block_tables.shape[1] if block_tables.dim() == 2 else 0
+    (rows, hq, d), qs = _query(query)
+    (nb, hkv, _, bd), bs = _bounds_strides(bounds)
+    width = _tables(block_tables, seq_lens, rows)
+    ss = scores.stride()
     if bd != d or hkv < 1 or hq % hkv:
         raise ValueError(f"{_WHO}: query {tuple(query.shape)} beside bounds {tuple(bounds.shape)}")
-    if scores.dtype != torch.float32 or tuple(scores.shape) != (rows, hkv, width) or (width > 1 and scores.stride(2) != 1):
+    if scores.dtype is not _F32 or scores.shape != (rows, hkv, width) or (width > 1 and ss[2] != 1):
         raise ValueError(f"{_WHO}: scores is {tuple(scores.shape)} {scores.dtype}; ({rows}, {hkv}, {width}) float32 with "
                          f"contiguous columns needed (the table's width)")
-    _tables(block_tables, seq_lens, rows)
     code = kv_dtype_code(kv_cache_dtype, bounds, query.dtype)
-    fp8 = code == _lib.KV_FP8_E4M3
-    scale = _positive(scale)
-    _need_cuda(scores, query, bounds, block_tables, seq_lens, k_scale)
-    _lib.check("hkb_page_scores", _lib.load().hkb_page_scores(
-        scores.data_ptr(), scores.stride(0), scores.stride(1), width, query.data_ptr(), query.stride(0), query.stride(1),
-        bounds.data_ptr(), bounds.stride(0), bounds.stride(1), nb, block_tables.data_ptr(), block_tables.stride(0),
-        seq_lens.data_ptr(), rows, hq, hkv, d, _page_size(block_size), scale, code,
-        _scale_ptr(k_scale, fp8, "k_scale"), _stream(query)))
+    scale, page = _positive(scale), _page_size(block_size)
+    stream = _on(query, scores, bounds, block_tables, seq_lens, k_scale)
+    rc = _lib.load().hkb_page_scores(
+        scores.data_ptr(), ss[0], ss[1], width, query.data_ptr(), qs[0], qs[1], bounds.data_ptr(), bs[0], bs[1], nb,
+        block_tables.data_ptr(), block_tables.stride(0), seq_lens.data_ptr(), rows, hq, hkv, d, page, scale, code,
+        _scale_ptr(k_scale, code == _lib.KV_FP8_E4M3, "k_scale"), stream)
+    if rc:
+        _lib.check("hkb_page_scores", rc)
     return scores
 
 
@@ -202,21 +251,24 @@ def select_pages(pages: torch.Tensor, scores: torch.Tensor, seq_lens: torch.Tens
     `first` and the `last` pages of the row's sequence and then those of the greatest `scores` (rows, kv_heads, columns)
     fp32, ties to the lowest page, NaN above all numbers. A row with no more pages than the budget gets them all.
     The entries number the row's pages (columns of its block table), as `paged_sparse_decode` reads them."""
-    _int32("pages", pages, 3)
-    _int32("seq_lens", seq_lens, 1)
+    _index("pages", pages, 3)
+    _index("seq_lens", seq_lens, 1)
     rows, hkv, budget = pages.shape
-    if scores.dtype != torch.float32 or scores.dim() != 3 or tuple(scores.shape[:2]) != (rows, hkv) \
-            or (scores.shape[2] > 1 and scores.stride(2) != 1):
-        raise ValueError(f"{_WHO}: scores is {tuple(scores.shape)} {scores.dtype} beside pages {tuple(pages.shape)}; "
+    shape, ss, ps = scores.shape, scores.stride(), pages.stride()
+    if scores.dtype is not _F32 or len(shape) != 3 or shape[0] != rows or shape[1] != hkv or (shape[2] > 1 and ss[2] != 1):
+        raise ValueError(f"{_WHO}: scores is {tuple(shape)} {scores.dtype} beside pages {tuple(pages.shape)}; "
                          f"({rows}, {hkv}, columns) float32 with contiguous columns needed")
     if seq_lens.shape[0] < rows:
         raise ValueError(f"{_WHO}: {seq_lens.shape[0]} lengths for {rows} rows")
     if first < 0 or last < 0 or first + last > budget:
         raise ValueError(f"{_WHO}: first {first} and last {last} pages of a budget of {budget}")
-    _need_cuda(pages, scores, seq_lens)
-    _lib.check("hkb_select_pages", _lib.load().hkb_select_pages(
-        pages.data_ptr(), pages.stride(0), pages.stride(1), budget, scores.data_ptr(), scores.stride(0), scores.stride(1),
-        scores.shape[2], seq_lens.data_ptr(), rows, hkv, _page_size(block_size), first, last, _stream(pages)))
+    page = _page_size(block_size)
+    stream = _on(pages, scores, seq_lens)
+    rc = _lib.load().hkb_select_pages(
+        pages.data_ptr(), ps[0], ps[1], budget, scores.data_ptr(), ss[0], ss[1], shape[2], seq_lens.data_ptr(), rows, hkv,
+        page, first, last, stream)
+    if rc:
+        _lib.check("hkb_select_pages", rc)
     return pages
 
 
@@ -230,30 +282,34 @@ def paged_sparse_decode(out: torch.Tensor, query: torch.Tensor, key_cache: torch
     twice. With nothing left a row answers zeros. `out_lse` (rows, q_heads) fp32 gets the natural-log sum-exp of the
     scaled scores (-inf for nothing), so that answers over disjoint pages can be merged (`merge_partials`). A NaN among
     a row's visible keys, or a logit outside fp32's range, makes the heads that meet it NaN."""
-    _query("query", query)
-    if out.shape != query.shape or out.dtype != query.dtype or out.stride(2) != 1:
-        raise ValueError(f"{_WHO}: out is {tuple(out.shape)} {out.dtype}; it must match query {tuple(query.shape)} {query.dtype}")
-    rows, hq, d = query.shape
-    if key_cache.dim() != 4 or value_cache.shape != key_cache.shape or key_cache.stride(3) != 1 or value_cache.stride(3) != 1 \
-            or key_cache.shape[3] != d or value_cache.dtype != key_cache.dtype:
-        raise ValueError(f"{_WHO}: key_cache {tuple(key_cache.shape)} {key_cache.dtype} / value_cache "
-                         f"{tuple(value_cache.shape)} {value_cache.dtype}; two (blocks, block_size, kv_heads, {d}) views "
-                         f"of one dtype needed")
-    _, page, hkv, _ = key_cache.shape
-    _tables(block_tables, seq_lens, rows)
-    _int32("pages", pages, 3)
-    if tuple(pages.shape[:2]) != (rows, hkv):
-        raise ValueError(f"{_WHO}: pages is {tuple(pages.shape)}; ({rows}, {hkv}, budget) needed")
-    if out_lse is not None and (out_lse.dtype != torch.float32 or tuple(out_lse.shape) != (rows, hq) or not out_lse.is_contiguous()):
-        raise ValueError(f"{_WHO}: out_lse is {tuple(out_lse.shape)} {out_lse.dtype}; contiguous ({rows}, {hq}) float32 needed")
+    qshape, qs = _query(query)
+    os = out.stride()
+    if out.shape != qshape or out.dtype is not query.dtype or os[2] != 1:
+        raise ValueError(f"{_WHO}: out is {tuple(out.shape)} {out.dtype} strides {tuple(os)}; it must match query "
+                         f"{tuple(qshape)} {query.dtype}")
+    rows, hq, d = qshape
+    (nb, page, hkv, cd), ks, vs = _cache_strides(key_cache, value_cache)
+    width = _tables(block_tables, seq_lens, rows)
+    _index("pages", pages, 3)
+    listed, heads, budget = pages.shape
+    ps = pages.stride()
+    if cd != d or listed != rows or heads != hkv:
+        raise ValueError(f"{_WHO}: pages is {tuple(pages.shape)} beside query {tuple(qshape)} and key_cache "
+                         f"{tuple(key_cache.shape)}; ({rows}, {hkv}, budget) and one head size needed")
+    lse = None
+    if out_lse is not None:
+        if out_lse.dtype is not _F32 or out_lse.shape != (rows, hq) or not out_lse.is_contiguous():
+            raise ValueError(f"{_WHO}: out_lse is {tuple(out_lse.shape)} {out_lse.dtype}; contiguous ({rows}, {hq}) float32 needed")
+        lse = out_lse.data_ptr()
     code = kv_dtype_code(kv_cache_dtype, key_cache, query.dtype)
     fp8 = code == _lib.KV_FP8_E4M3
     scale = _positive(scale)
-    _need_cuda(out, query, key_cache, value_cache, block_tables, seq_lens, pages, k_scale, v_scale, out_lse)
-    _lib.check("hkb_paged_sparse_decode", _lib.load().hkb_paged_sparse_decode(
-        out.data_ptr(), out.stride(0), out.stride(1), out_lse.data_ptr() if out_lse is not None else None,
-        query.data_ptr(), query.stride(0), query.stride(1), _cache_t(key_cache), _cache_t(value_cache),
-        block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], seq_lens.data_ptr(),
-        pages.data_ptr(), pages.stride(0), pages.stride(1), pages.shape[2], rows, hq, hkv, d, page, scale, code,
-        _scale_ptr(k_scale, fp8, "k_scale"), _scale_ptr(v_scale, fp8, "v_scale"), _stream(query)))
+    stream = _on(query, out, key_cache, value_cache, block_tables, seq_lens, pages, k_scale, v_scale, out_lse)
+    rc = _lib.load().hkb_paged_sparse_decode(
+        out.data_ptr(), os[0], os[1], lse, query.data_ptr(), qs[0], qs[1],
+        _lib.CacheT(key_cache.data_ptr(), ks[0], ks[1], ks[2], nb), _lib.CacheT(value_cache.data_ptr(), vs[0], vs[1], vs[2], nb),
+        block_tables.data_ptr(), block_tables.stride(0), width, seq_lens.data_ptr(), pages.data_ptr(), ps[0], ps[1], budget,
+        rows, hq, hkv, d, page, scale, code, _scale_ptr(k_scale, fp8, "k_scale"), _scale_ptr(v_scale, fp8, "v_scale"), stream)
+    if rc:
+        _lib.check("hkb_paged_sparse_decode", rc)
     return out
