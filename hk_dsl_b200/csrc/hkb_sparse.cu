@@ -6,11 +6,11 @@
 //
 // Bound: bytes (the selected K and V rows once, 4 to 16 flop a byte). A cluster of `splits` CTAs takes a (row, kv
 // head); the 16-token tiles of its pages are dealt to all the cluster's warps in turn, each warp a cp.async ring and
-// an online softmax of its own (the decode walk's workers, fragments and all). The warps' normalised partials stay
+// an online softmax of its own (SparseWorker). The warps' normalised partials stay
 // in shared memory, and after one cluster barrier every CTA folds its slice of the outputs out of its peers' memory:
 // one launch, no scratch, nothing shared between calls.
 #include "hkb_cluster.cuh"
-#include "hkb_walk_mma.cuh"
+#include "hkb_sparse.cuh"
 
 namespace hkb {
 
@@ -26,6 +26,7 @@ template <class P, int WARPS, bool F16>
 __global__ void __launch_bounds__(WARPS * 32) sparse_kernel(const SparseArgs a) {
   extern __shared__ __align__(128) uint8_t hkb_smem[];
   constexpr int D = P::HEAD_DIM, HEADS = P::HEADS, NST = P::STAGES;
+  static_assert(NST >= 2, "a stage is computed on while the next is fetched");
   static_assert(HEADS * (D + 1) * 4 <= P::RING_SMEM, "a warp's partial lies where its ring was");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ctas = cluster_size(), rank = cluster_rank();
@@ -67,32 +68,34 @@ __global__ void __launch_bounds__(WARPS * 32) sparse_kernel(const SparseArgs a) 
   const uint32_t ring = smem_u32(hkb_smem) + warp * P::RING_SMEM;
   // Requests the warp's next tile into a ring stage; its first token, or -1 where none is left.
   auto issue = [&](int stage) -> int {
-    while (!live) {
-      if ((int64_t)(next_item - 32) * workers >= total) return -1;
+    int t = -1;
+    while (!live && (int64_t)(next_item - 32) * workers < total) {
       id = id_n; tok = tok_n;
       live = __ballot_sync(0xffffffffu, tok >= 0);
       look_up(next_item, id_n, tok_n);
       next_item += 32;
     }
-    const int src = __ffs(live) - 1;
-    live &= live - 1;
-    const int t = __shfl_sync(0xffffffffu, tok, src);
-    ld.issue(ring + stage * P::STAGE_BYTES, t / TILE_TOKENS, __shfl_sync(0xffffffffu, id, src), lane);
+    if (live) {
+      const int src = __ffs(live) - 1;
+      live &= live - 1;
+      t = __shfl_sync(0xffffffffu, tok, src);
+      ld.issue(ring + stage * P::STAGE_BYTES, t / TILE_TOKENS, __shfl_sync(0xffffffffu, id, src), lane);
+    }
+    cp_async_commit();
     return t;
   };
   int queue[NST - 1];            // first tokens of the tiles in flight, oldest first
 #pragma unroll
-  for (int k = 0; k < NST - 1; ++k) { queue[k] = issue(k); cp_async_commit(); }
+  for (int k = 0; k < NST - 1; ++k) queue[k] = issue(k);
 
   typename P::State st;
-  P::begin(st, a.d, row, hq0, nh, lane, qs);
+  P::Walk::begin(st, a.d, row, hq0, nh, lane, qs);
   int sc = 0, sl = NST - 1;
   while (queue[0] >= 0) {
     cp_async_wait<NST - 2>();
     __syncwarp();
-    const int t = issue(sl);
-    cp_async_commit();
-    P::step(st, ring, sc, queue[0], seq_len, queue[0] + TILE_TOKENS > seq_len, lane, qs);
+    const int t = issue(sl);     // over the tile before
+    P::step(st, ring + sc * P::STAGE_BYTES, queue[0], seq_len, queue[0] + TILE_TOKENS > seq_len, lane, qs);
 #pragma unroll
     for (int k = 0; k + 1 < NST - 1; ++k) queue[k] = queue[k + 1];
     queue[NST - 2] = t;
@@ -104,7 +107,7 @@ __global__ void __launch_bounds__(WARPS * 32) sparse_kernel(const SparseArgs a) 
 
   // The warp's partial over its ring: [head][D] normalised, then [head] lse.
   float* part = reinterpret_cast<float*>(hkb_smem + warp * P::RING_SMEM);
-  P::end(st, lane, nh, vs, part, part + HEADS * D);
+  P::Walk::end(st, lane, nh, vs, part, part + HEADS * D);
   // a NaN among the scores makes the sum NaN: the partial says so instead of counting as empty
 #pragma unroll
   for (int nt = 0; nt < HEADS / 8; ++nt)
@@ -175,9 +178,33 @@ __global__ void __launch_bounds__(WARPS * 32) sparse_kernel(const SparseArgs a) 
   if (ctas > 1) cluster_sync();  // no CTA leaves while a peer reads its memory
 }
 
-template <class P, int WARPS, bool F16>
+// How many CTAs, of how many warps, share a (row, kv head). Two warps a CTA, so that many fit an SM and one's first
+// and last trips to memory lie under its neighbours' streams, and as many CTAs as the machine holds at once, up to the
+// portable cluster: more only adds waves of them (each costs about 6 us whatever it does), fewer leave a batch of few
+// rows to few warps. Where even eight CTAs of two warps leave half the machine's mma pipes idle and each warp has more
+// than eight tiles to go, four warps a CTA. Measured at head size 128, 16-token pages, us:
+//   bf16, 64 x 8 items of 64 pages: 1 CTA 45.5, 2 48.4, 4 55.8 (two warps); 1 CTA of four 46.9, of eight 53.0
+//   bf16, 16 x 8 items of 256 pages: 1 CTA 67.0, 2 47.6, 4 45.7, 8 49.5; 2 x 8 of 1024: 8 CTAs 37.0, of four warps 28.4
+//   fp8, 48 x 8 items of 64 pages (rings half the size, so twice the CTAs fit): 1 CTA 29.1, 2 22.6, 4 28.9
+// Short lists do not pay for the wider clusters: fp8, 16 x 8 items of 16 pages: 4 CTAs 7.1, 8 8.5.
+struct SparseShape { int ctas, warps; };
+static SparseShape sparse_shape(int rows, int kv_heads, int64_t tiles, int ring_bytes) {
+  int sms = hkb_sm_count(-1);
+  if (sms <= 0) sms = 148;
+  SparseShape s = {1, 2};
+  const int64_t items = (int64_t)rows * kv_heads;
+  int fit = (227 << 10) / (2 * ring_bytes + 1024);
+  fit = fit > 8 ? 8 : fit;
+  if (tiles < 64 && fit > 4) fit = 4;
+  while (s.ctas < 8 && items * s.ctas * 2 <= (int64_t)fit * sms && tiles > s.ctas * 2) s.ctas *= 2;
+  if (s.ctas == 8 && items * 8 <= 2 * sms && tiles > 128) s.warps = 4;
+  return s;
+}
+
+template <int D, int KIND, int NT, int NST, int WARPS>
 static int launch_sparse(const SparseArgs& a, int rows, int splits, cudaStream_t st) {
-  auto kernel = sparse_kernel<P, WARPS, F16>;
+  using P = SparseWorker<D, KIND, NT, NST>;
+  auto kernel = sparse_kernel<P, WARPS, KIND == HKB_KV_F16>;
   constexpr int smem = WARPS * P::RING_SMEM;
   static bool armed[64] = {};    // more than 48 KB of shared memory: asked for once a device
   int dev = 0;
@@ -190,25 +217,20 @@ static int launch_sparse(const SparseArgs& a, int rows, int splits, cudaStream_t
   return launch_cluster((const void*)kernel, dim3(splits, a.d.num_kv_heads, rows), WARPS * 32, splits, smem, &a, st);
 }
 
-template <int D, bool F16>
-static int dispatch_sparse16(const SparseArgs& a, int rows, int splits, cudaStream_t st) {
-  constexpr int NST = D == 256 ? 2 : 3;
-  if (a.d.group <= 8) return launch_sparse<WalkMMA<D, false, 1, 4, NST, F16>, 4, F16>(a, rows, splits, st);
-  return launch_sparse<WalkMMA<D, false, 2, 4, NST, F16>, 4, F16>(a, rows, splits, st);
+template <int D, int KIND, int NT>
+static int dispatch_sparse(const SparseArgs& a, int rows, cudaStream_t st) {
+  constexpr int NST = D == 256 && KIND != HKB_KV_FP8_E4M3 ? 2 : 3;      // a 16-bit tile of head size 256 is 16 KB
+  const SparseShape shape = sparse_shape(rows, a.d.num_kv_heads, (int64_t)a.budget * a.d.tiles_per_page, SparseWorker<D, KIND, NT, NST>::RING_SMEM);
+  return shape.warps == 2 ? launch_sparse<D, KIND, NT, NST, 2>(a, rows, shape.ctas, st) : launch_sparse<D, KIND, NT, NST, 4>(a, rows, shape.ctas, st);
 }
-template <int D>
-static int dispatch_sparse8(const SparseArgs& a, int rows, int splits, cudaStream_t st) {
-  if (a.d.group <= 8) return launch_sparse<WalkMMAF8<D, 1, 3, 1>, 4, false>(a, rows, splits, st);
-  return launch_sparse<WalkMMAF8<D, 2, 3, 1>, 4, false>(a, rows, splits, st);
+template <int KIND, int NT>
+static int dispatch_sparse_dim(const SparseArgs& a, int head_dim, int rows, cudaStream_t st) {
+  if (head_dim == 64) return dispatch_sparse<64, KIND, NT>(a, rows, st);
+  return head_dim == 128 ? dispatch_sparse<128, KIND, NT>(a, rows, st) : dispatch_sparse<256, KIND, NT>(a, rows, st);
 }
-
-// How many CTAs share a (row, kv head).
-static int sparse_splits(int rows, int kv_heads, int64_t tiles) {
-  int sms = hkb_sm_count(-1);
-  if (sms <= 0) sms = 148;
-  int c = 1;
-  while (c < 8 && (int64_t)rows * kv_heads * c < 2 * sms && tiles > c * 8) c *= 2;
-  return c;
+template <int KIND>
+static int dispatch_sparse_group(const SparseArgs& a, int head_dim, int rows, cudaStream_t st) {
+  return a.d.group <= 8 ? dispatch_sparse_dim<KIND, 1>(a, head_dim, rows, st) : dispatch_sparse_dim<KIND, 2>(a, head_dim, rows, st);
 }
 
 }  // namespace hkb
@@ -255,16 +277,8 @@ extern "C" int hkb_paged_sparse_decode(void* out, int64_t out_stride_tok, int64_
   a.scale = scale; a.k_scale = fp8 ? k_scale : nullptr; a.v_scale = fp8 ? v_scale : nullptr;
   s.pages = pages; s.p_stride_row = pages_stride_row; s.p_stride_head = pages_stride_head; s.budget = budget;
   s.out_lse = out_lse;
-  const int splits = sparse_splits(num_rows, num_kv_heads, (int64_t)budget * a.tiles_per_page);
   cudaStream_t st = (cudaStream_t)stream;
-  if (kv_dtype == HKB_KV_F16) {
-    if (head_dim == 128) return dispatch_sparse16<128, true>(s, num_rows, splits, st);
-    return head_dim == 256 ? dispatch_sparse16<256, true>(s, num_rows, splits, st) : dispatch_sparse16<64, true>(s, num_rows, splits, st);
-  }
-  if (fp8) {
-    if (head_dim == 128) return dispatch_sparse8<128>(s, num_rows, splits, st);
-    return head_dim == 256 ? dispatch_sparse8<256>(s, num_rows, splits, st) : dispatch_sparse8<64>(s, num_rows, splits, st);
-  }
-  if (head_dim == 128) return dispatch_sparse16<128, false>(s, num_rows, splits, st);
-  return head_dim == 256 ? dispatch_sparse16<256, false>(s, num_rows, splits, st) : dispatch_sparse16<64, false>(s, num_rows, splits, st);
+  if (kv_dtype == HKB_KV_F16) return dispatch_sparse_group<HKB_KV_F16>(s, head_dim, num_rows, st);
+  if (fp8) return dispatch_sparse_group<HKB_KV_FP8_E4M3>(s, head_dim, num_rows, st);
+  return dispatch_sparse_group<HKB_KV_BF16>(s, head_dim, num_rows, st);
 }

@@ -69,8 +69,10 @@ def _page_size(block_size: int) -> int:
 
 def _tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, rows: int) -> int:
     """The checked table's width."""
-    _index("block_tables", block_tables, 2)
-    _index("seq_lens", seq_lens, 1)
+    if block_tables.dtype is not _I32 or seq_lens.dtype is not _I32 or block_tables.dim() != 2 or seq_lens.dim() != 1 \
+            or not block_tables.is_contiguous() or not seq_lens.is_contiguous():
+        _index("block_tables", block_tables, 2)       # which of them, and whether a strided one is one the kernels take
+        _index("seq_lens", seq_lens, 1)
     have, width = block_tables.shape
     if have < rows or seq_lens.shape[0] < rows:
         raise ValueError(f"{_WHO}: block_tables {tuple(block_tables.shape)} and seq_lens {tuple(seq_lens.shape)} "
@@ -200,6 +202,13 @@ def update_page_bounds(bounds: torch.Tensor, key_cache: torch.Tensor, block_tabl
     return bounds
 
 
+def _code(kv_cache_dtype: str, cache: torch.Tensor, dtype) -> int:
+    """`kv_dtype_code`, the common case first: a 16-bit cache of the query's own type."""
+    if kv_cache_dtype == "auto" and cache.dtype is dtype:
+        return _lib.KV_BF16 if dtype is _BF16 else _lib.KV_F16
+    return kv_dtype_code(kv_cache_dtype, cache, dtype)
+
+
 def _positive(scale: float) -> float:
     scale = float(scale)
     if not scale > 0.0:
@@ -233,7 +242,7 @@ def page_scores(scores: torch.Tensor, query: torch.Tensor, bounds: torch.Tensor,
     if scores.dtype is not _F32 or scores.shape != (rows, hkv, width) or (width > 1 and ss[2] != 1):
         raise ValueError(f"{_WHO}: scores is {tuple(scores.shape)} {scores.dtype}; ({rows}, {hkv}, {width}) float32 with "
                          f"contiguous columns needed (the table's width)")
-    code = kv_dtype_code(kv_cache_dtype, bounds, query.dtype)
+    code = _code(kv_cache_dtype, bounds, query.dtype)
     scale, page = _positive(scale), _page_size(block_size)
     stream = _on(query, scores, bounds, block_tables, seq_lens, k_scale)
     rc = _lib.load().hkb_page_scores(
@@ -301,7 +310,7 @@ def paged_sparse_decode(out: torch.Tensor, query: torch.Tensor, key_cache: torch
         if out_lse.dtype is not _F32 or out_lse.shape != (rows, hq) or not out_lse.is_contiguous():
             raise ValueError(f"{_WHO}: out_lse is {tuple(out_lse.shape)} {out_lse.dtype}; contiguous ({rows}, {hq}) float32 needed")
         lse = out_lse.data_ptr()
-    code = kv_dtype_code(kv_cache_dtype, key_cache, query.dtype)
+    code = _code(kv_cache_dtype, key_cache, query.dtype)
     fp8 = code == _lib.KV_FP8_E4M3
     scale = _positive(scale)
     stream = _on(query, out, key_cache, value_cache, block_tables, seq_lens, pages, k_scale, v_scale, out_lse)
