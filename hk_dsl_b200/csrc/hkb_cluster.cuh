@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "../../include/hkb.h"
 
 extern thread_local int hkb_tls_cuda_error;
@@ -39,6 +41,13 @@ __device__ __forceinline__ float peer_f1(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
   return v;
+}
+
+// Whether 64-bit arguments are all ints.
+inline bool ints(std::initializer_list<int64_t> values) {
+  for (int64_t v : values)
+    if (v < -0x80000000LL || v > 0x7fffffffLL) return false;
+  return true;
 }
 
 // One argument struct, `cluster` CTAs of grid.x a cluster (1: an ordinary launch; past 8, the portable size,

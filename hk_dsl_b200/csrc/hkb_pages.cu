@@ -926,13 +926,10 @@ static int launch_scores(const ScoreArgs& a, dim3 grid, cudaStream_t st) {
   return launched([&] { scores_kernel<KIND, D, NT><<<grid, SCORE_WARPS * 32, smem, st>>>(a); });
 }
 
-}  // namespace hkb
-
-extern "C" int hkb_advance_tables(int32_t* block_table, int64_t table_stride, int max_pages, int32_t* seq_lens,
+static int advance_tables(int32_t* block_table, int64_t table_stride, int max_pages, int32_t* seq_lens,
                                   const int32_t* new_tokens, int num_reqs, int block_size, int32_t* free_pages,
                                   int64_t free_capacity, int32_t* free_count, int64_t* slot_mapping, int64_t* positions,
                                   int64_t num_rows, int32_t* q_start, int32_t* status, void* stream) {
-  using namespace hkb;
   if (num_reqs < 0 || max_pages < 0 || free_capacity < 0 || num_rows < 0 ||
       free_capacity > 0x7fffffff || num_rows > 0x40000000 || num_reqs > 0x40000000) return HKB_ERR_SIZE;
   if (block_size <= 0) return HKB_ERR_BLOCK_SIZE;
@@ -961,13 +958,12 @@ extern "C" int hkb_advance_tables(int32_t* block_table, int64_t table_stride, in
   return launch_cluster((const void*)advance_kernel<8, 2>, dim3(1), 256, 1, 0, &a, (cudaStream_t)stream);
 }
 
-extern "C" int hkb_page_bounds(void* bounds, int64_t bounds_stride_block, int64_t bounds_stride_head, int64_t bounds_blocks,
+static int page_bounds(void* bounds, int64_t bounds_stride_block, int64_t bounds_stride_head, int64_t bounds_blocks,
                                hkb_cache_t kc, const int32_t* block_table, int64_t table_stride, int max_pages,
                                const int32_t* seq_lens, const int32_t* q_start, int num_seqs, int64_t num_tokens,
                                int num_kv_heads, int head_dim, int block_size, int kv_dtype, void* stream) {
-  using namespace hkb;
   if (num_seqs < 0 || num_kv_heads <= 0 || max_pages < 0 || kc.num_blocks < 0 || bounds_blocks < 0 || num_tokens < 0) return HKB_ERR_SIZE;
-  if (num_seqs == 0 || max_pages == 0 || (q_start && num_tokens == 0)) return HKB_OK;
+  if (num_seqs == 0 || max_pages == 0) return HKB_OK;
   if (!bounds || !kc.ptr || !block_table || !seq_lens) return HKB_ERR_NULL;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return HKB_ERR_HEAD_DIM;
   if (block_size <= 0) return HKB_ERR_BLOCK_SIZE;
@@ -1002,13 +998,12 @@ extern "C" int hkb_page_bounds(void* bounds, int64_t bounds_stride_block, int64_
   });
 }
 
-extern "C" int hkb_page_scores(float* scores, int64_t scores_stride_row, int64_t scores_stride_head, int num_columns,
+static int page_scores(float* scores, int64_t scores_stride_row, int64_t scores_stride_head, int num_columns,
                                const void* q, int64_t q_stride_row, int64_t q_stride_head,
                                const void* bounds, int64_t bounds_stride_block, int64_t bounds_stride_head,
                                int64_t bounds_blocks, const int32_t* block_table, int64_t table_stride,
                                const int32_t* seq_lens, int num_rows, int num_q_heads, int num_kv_heads, int head_dim,
                                int block_size, float scale, int kv_dtype, const float* k_scale, void* stream) {
-  using namespace hkb;
   if (num_rows < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_columns < 0 || num_rows > 65535 || num_kv_heads > 65535) return HKB_ERR_SIZE;
   if (num_rows == 0 || num_columns == 0) return HKB_OK;
   if (!scores || !q || !bounds || !block_table || !seq_lens) return HKB_ERR_NULL;
@@ -1049,11 +1044,10 @@ extern "C" int hkb_page_scores(float* scores, int64_t scores_stride_row, int64_t
   return HKB_ERR_UNSUPPORTED;
 }
 
-extern "C" int hkb_select_pages(int32_t* pages, int64_t pages_stride_row, int64_t pages_stride_head, int budget,
+static int select_pages(int32_t* pages, int64_t pages_stride_row, int64_t pages_stride_head, int budget,
                                 const float* scores, int64_t scores_stride_row, int64_t scores_stride_head, int num_columns,
                                 const int32_t* seq_lens, int num_rows, int num_kv_heads, int block_size, int first, int last,
                                 void* stream) {
-  using namespace hkb;
   if (num_rows < 0 || num_kv_heads <= 0 || num_kv_heads > 65535 || num_columns < 0 || budget < 0 || first < 0 || last < 0 ||
       (int64_t)first + last > budget) return HKB_ERR_SIZE;
   if (num_rows == 0 || budget == 0) return HKB_OK;
@@ -1064,10 +1058,11 @@ extern "C" int hkb_select_pages(int32_t* pages, int64_t pages_stride_row, int64_
   a.pages = pages; a.p_stride_row = pages_stride_row; a.p_stride_head = pages_stride_head; a.budget = budget;
   a.scores = scores; a.s_stride_row = scores_stride_row; a.s_stride_head = scores_stride_head; a.columns = num_columns;
   a.seq_lens = seq_lens; a.page = block_size; a.first = first; a.last = last;
+  const int64_t items = (int64_t)num_rows * num_kv_heads;
+  if (items > 0x7fffffff) return HKB_ERR_SIZE;
   const dim3 grid(num_rows, num_kv_heads);
   cudaStream_t st = (cudaStream_t)stream;
   return launched([&] {
-    const int64_t items = (int64_t)num_rows * num_kv_heads;
     const unsigned ctas = (unsigned)((items + SELECT_WARPS - 1) / SELECT_WARPS);
     if (num_columns <= 256) select_warp_kernel<8><<<ctas, SELECT_WARPS * 32, 0, st>>>(a, num_kv_heads, items);
     else if (num_columns <= 512) select_warp_kernel<16><<<ctas, SELECT_WARPS * 32, 0, st>>>(a, num_kv_heads, items);
@@ -1077,4 +1072,40 @@ extern "C" int hkb_select_pages(int32_t* pages, int64_t pages_stride_row, int64_
     else if (num_columns <= 16384) select_kernel<1024, 16, true><<<grid, 1024, 0, st>>>(a);
     else select_kernel<1024, 16, false><<<grid, 1024, 0, st>>>(a);
   });
+}
+
+}  // namespace hkb
+
+extern "C" int hkb_advance_tables(const hkb_advance_t* p, void* stream) {
+  if (!p) return HKB_ERR_NULL;
+  if (!hkb::ints({p->max_pages, p->num_reqs, p->block_size})) return HKB_ERR_SIZE;
+  return hkb::advance_tables(p->block_table, p->table_stride, (int)p->max_pages, p->seq_lens, p->new_tokens, (int)p->num_reqs,
+                             (int)p->block_size, p->free_pages, p->free_capacity, p->free_count, p->slot_mapping,
+                             p->positions, p->num_rows, p->q_start, p->status, stream);
+}
+
+extern "C" int hkb_page_bounds(const hkb_page_bounds_t* p, void* stream) {
+  if (!p) return HKB_ERR_NULL;
+  if (!hkb::ints({p->max_pages, p->num_seqs, p->num_kv_heads, p->head_dim, p->block_size, p->kv_dtype})) return HKB_ERR_SIZE;
+  return hkb::page_bounds(p->bounds, p->bounds_stride_block, p->bounds_stride_head, p->bounds_blocks, p->k_cache,
+                          p->block_table, p->table_stride, (int)p->max_pages, p->seq_lens, p->q_start, (int)p->num_seqs,
+                          p->num_tokens, (int)p->num_kv_heads, (int)p->head_dim, (int)p->block_size, (int)p->kv_dtype, stream);
+}
+
+extern "C" int hkb_page_scores(const hkb_page_scores_t* p, void* stream) {
+  if (!p) return HKB_ERR_NULL;
+  if (!hkb::ints({p->num_columns, p->num_rows, p->num_q_heads, p->num_kv_heads, p->head_dim, p->block_size, p->kv_dtype})) return HKB_ERR_SIZE;
+  return hkb::page_scores(p->scores, p->scores_stride_row, p->scores_stride_head, (int)p->num_columns, p->q, p->q_stride_row,
+                          p->q_stride_head, p->bounds, p->bounds_stride_block, p->bounds_stride_head, p->bounds_blocks,
+                          p->block_table, p->table_stride, p->seq_lens, (int)p->num_rows, (int)p->num_q_heads,
+                          (int)p->num_kv_heads, (int)p->head_dim, (int)p->block_size, (float)p->scale, (int)p->kv_dtype,
+                          p->k_scale, stream);
+}
+
+extern "C" int hkb_select_pages(const hkb_select_pages_t* p, void* stream) {
+  if (!p) return HKB_ERR_NULL;
+  if (!hkb::ints({p->budget, p->num_columns, p->num_rows, p->num_kv_heads, p->block_size, p->first, p->last})) return HKB_ERR_SIZE;
+  return hkb::select_pages(p->pages, p->pages_stride_row, p->pages_stride_head, (int)p->budget, p->scores,
+                           p->scores_stride_row, p->scores_stride_head, (int)p->num_columns, p->seq_lens, (int)p->num_rows,
+                           (int)p->num_kv_heads, (int)p->block_size, (int)p->first, (int)p->last, stream);
 }

@@ -233,16 +233,13 @@ static int dispatch_sparse_group(const SparseArgs& a, int head_dim, int rows, cu
   return a.d.group <= 8 ? dispatch_sparse_dim<KIND, 1>(a, head_dim, rows, st) : dispatch_sparse_dim<KIND, 2>(a, head_dim, rows, st);
 }
 
-}  // namespace hkb
-
-extern "C" int hkb_paged_sparse_decode(void* out, int64_t out_stride_tok, int64_t out_stride_head, float* out_lse,
+static int sparse_decode(void* out, int64_t out_stride_tok, int64_t out_stride_head, float* out_lse,
                                        const void* q, int64_t q_stride_tok, int64_t q_stride_head,
                                        hkb_cache_t kc, hkb_cache_t vc, const int32_t* block_table, int64_t table_stride,
                                        int max_pages, const int32_t* seq_lens, const int32_t* pages,
                                        int64_t pages_stride_row, int64_t pages_stride_head, int budget, int num_rows,
                                        int num_q_heads, int num_kv_heads, int head_dim, int block_size, float scale,
                                        int kv_dtype, const float* k_scale, const float* v_scale, void* stream) {
-  using namespace hkb;
   if (num_rows < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || max_pages < 0 || budget < 0) return HKB_ERR_SIZE;
   if (num_rows == 0) return HKB_OK;
   if (num_rows > 65535 || num_kv_heads > 65535) return HKB_ERR_SIZE;
@@ -281,4 +278,17 @@ extern "C" int hkb_paged_sparse_decode(void* out, int64_t out_stride_tok, int64_
   if (kv_dtype == HKB_KV_F16) return dispatch_sparse_group<HKB_KV_F16>(s, head_dim, num_rows, st);
   if (fp8) return dispatch_sparse_group<HKB_KV_FP8_E4M3>(s, head_dim, num_rows, st);
   return dispatch_sparse_group<HKB_KV_BF16>(s, head_dim, num_rows, st);
+}
+
+}  // namespace hkb
+
+extern "C" int hkb_paged_sparse_decode(const hkb_sparse_decode_t* p, void* stream) {
+  if (!p) return HKB_ERR_NULL;
+  if (!hkb::ints({p->max_pages, p->budget, p->num_rows, p->num_q_heads, p->num_kv_heads, p->head_dim, p->block_size, p->kv_dtype}))
+    return HKB_ERR_SIZE;
+  return hkb::sparse_decode(p->out, p->out_stride_tok, p->out_stride_head, p->out_lse, p->q, p->q_stride_tok, p->q_stride_head,
+                            p->k_cache, p->v_cache, p->block_table, p->table_stride, (int)p->max_pages, p->seq_lens, p->pages,
+                            p->pages_stride_row, p->pages_stride_head, (int)p->budget, (int)p->num_rows, (int)p->num_q_heads,
+                            (int)p->num_kv_heads, (int)p->head_dim, (int)p->block_size, (float)p->scale, (int)p->kv_dtype,
+                            p->k_scale, p->v_scale, stream);
 }

@@ -102,12 +102,11 @@ def advance_tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, new_token
     with `REQ_NO_PAGES` (too few free pages; once one is short, so is every later one that needs any), `REQ_TABLE_FULL`
     or `REQ_NO_ROWS` keeps its length, gets no page, and its rows get slot -1. A page belongs to one request."""
     _index("block_tables", block_tables, 2)
-    _index("seq_lens", seq_lens, 1)
-    _index("new_tokens", new_tokens, 1)
-    _index("free_pages", free_pages, 1)
-    _index("free_count", free_count, 1)
-    _index("query_start_loc", query_start_loc, 1)
-    _index("status", status, 1)
+    for t in (seq_lens, new_tokens, free_pages, free_count, query_start_loc, status):
+        if t.dtype is not _I32 or t.dim() != 1 or not t.is_contiguous():
+            for name, x in (("seq_lens", seq_lens), ("new_tokens", new_tokens), ("free_pages", free_pages),
+                            ("free_count", free_count), ("query_start_loc", query_start_loc), ("status", status)):
+                _index(name, x, 1)
     _index("slot_mapping", slot_mapping, 1, _I64)
     _index("positions", positions, 1, _I64)
     n, = seq_lens.shape
@@ -125,10 +124,10 @@ def advance_tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, new_token
         raise ValueError(f"{_WHO}: block_tables' rows overlap (strides {tuple(block_tables.stride())}); it is written")
     page = _page_size(block_size)
     stream = _on(seq_lens, block_tables, new_tokens, free_pages, free_count, slot_mapping, positions, query_start_loc, status)
-    rc = _lib.load().hkb_advance_tables(
+    rc = _lib.load().hkb_advance_tables(_lib.ADVANCE(
         block_tables.data_ptr(), stride, width, seq_lens.data_ptr(), new_tokens.data_ptr(), n, page,
         free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), slot_mapping.data_ptr(), positions.data_ptr(),
-        rows, query_start_loc.data_ptr(), status.data_ptr(), stream)
+        rows, query_start_loc.data_ptr(), status.data_ptr()), stream)
     if rc:
         _lib.check("hkb_advance_tables", rc)
 
@@ -184,7 +183,7 @@ def update_page_bounds(bounds: torch.Tensor, key_cache: torch.Tensor, block_tabl
                          f"{key_cache.dtype}")
     n = seq_lens.shape[0]
     width = _tables(block_tables, seq_lens, n)
-    starts = None
+    starts = 0
     if query_start_loc is not None:
         _index("query_start_loc", query_start_loc, 1)
         if query_start_loc.shape[0] < n + 1:
@@ -193,10 +192,10 @@ def update_page_bounds(bounds: torch.Tensor, key_cache: torch.Tensor, block_tabl
             raise ValueError(f"{_WHO}: query_start_loc needs num_tokens, the rows of the step (a host number), not {num_tokens}")
         starts = query_start_loc.data_ptr()
     stream = _on(bounds, key_cache, block_tables, seq_lens, query_start_loc)
-    rc = _lib.load().hkb_page_bounds(
-        bounds.data_ptr(), bs[0], bs[1], bshape[0], _lib.CacheT(key_cache.data_ptr(), ks[0], ks[1], ks[2], nb),
+    rc = _lib.load().hkb_page_bounds(_lib.PAGE_BOUNDS(
+        bounds.data_ptr(), bs[0], bs[1], bshape[0], key_cache.data_ptr(), ks[0], ks[1], ks[2], nb,
         block_tables.data_ptr(), block_tables.stride(0), width, seq_lens.data_ptr(), starts, n, num_tokens or 0, hkv, d,
-        page, code, stream)
+        page, code), stream)
     if rc:
         _lib.check("hkb_page_bounds", rc)
     return bounds
@@ -245,10 +244,10 @@ def page_scores(scores: torch.Tensor, query: torch.Tensor, bounds: torch.Tensor,
     code = _code(kv_cache_dtype, bounds, query.dtype)
     scale, page = _positive(scale), _page_size(block_size)
     stream = _on(query, scores, bounds, block_tables, seq_lens, k_scale)
-    rc = _lib.load().hkb_page_scores(
+    rc = _lib.load().hkb_page_scores(_lib.PAGE_SCORES(
         scores.data_ptr(), ss[0], ss[1], width, query.data_ptr(), qs[0], qs[1], bounds.data_ptr(), bs[0], bs[1], nb,
-        block_tables.data_ptr(), block_tables.stride(0), seq_lens.data_ptr(), rows, hq, hkv, d, page, scale, code,
-        _scale_ptr(k_scale, code == _lib.KV_FP8_E4M3, "k_scale"), stream)
+        block_tables.data_ptr(), block_tables.stride(0), seq_lens.data_ptr(), rows, hq, hkv, d, page, code,
+        _scale_ptr(k_scale, code == _lib.KV_FP8_E4M3, "k_scale") or 0, scale), stream)
     if rc:
         _lib.check("hkb_page_scores", rc)
     return scores
@@ -273,9 +272,9 @@ def select_pages(pages: torch.Tensor, scores: torch.Tensor, seq_lens: torch.Tens
         raise ValueError(f"{_WHO}: first {first} and last {last} pages of a budget of {budget}")
     page = _page_size(block_size)
     stream = _on(pages, scores, seq_lens)
-    rc = _lib.load().hkb_select_pages(
+    rc = _lib.load().hkb_select_pages(_lib.SELECT_PAGES(
         pages.data_ptr(), ps[0], ps[1], budget, scores.data_ptr(), ss[0], ss[1], shape[2], seq_lens.data_ptr(), rows, hkv,
-        page, first, last, stream)
+        page, first, last), stream)
     if rc:
         _lib.check("hkb_select_pages", rc)
     return pages
@@ -305,7 +304,7 @@ def paged_sparse_decode(out: torch.Tensor, query: torch.Tensor, key_cache: torch
     if cd != d or listed != rows or heads != hkv:
         raise ValueError(f"{_WHO}: pages is {tuple(pages.shape)} beside query {tuple(qshape)} and key_cache "
                          f"{tuple(key_cache.shape)}; ({rows}, {hkv}, budget) and one head size needed")
-    lse = None
+    lse = 0
     if out_lse is not None:
         if out_lse.dtype is not _F32 or out_lse.shape != (rows, hq) or not out_lse.is_contiguous():
             raise ValueError(f"{_WHO}: out_lse is {tuple(out_lse.shape)} {out_lse.dtype}; contiguous ({rows}, {hq}) float32 needed")
@@ -314,11 +313,12 @@ def paged_sparse_decode(out: torch.Tensor, query: torch.Tensor, key_cache: torch
     fp8 = code == _lib.KV_FP8_E4M3
     scale = _positive(scale)
     stream = _on(query, out, key_cache, value_cache, block_tables, seq_lens, pages, k_scale, v_scale, out_lse)
-    rc = _lib.load().hkb_paged_sparse_decode(
+    rc = _lib.load().hkb_paged_sparse_decode(_lib.SPARSE_DECODE(
         out.data_ptr(), os[0], os[1], lse, query.data_ptr(), qs[0], qs[1],
-        _lib.CacheT(key_cache.data_ptr(), ks[0], ks[1], ks[2], nb), _lib.CacheT(value_cache.data_ptr(), vs[0], vs[1], vs[2], nb),
+        key_cache.data_ptr(), ks[0], ks[1], ks[2], nb, value_cache.data_ptr(), vs[0], vs[1], vs[2], nb,
         block_tables.data_ptr(), block_tables.stride(0), width, seq_lens.data_ptr(), pages.data_ptr(), ps[0], ps[1], budget,
-        rows, hq, hkv, d, page, scale, code, _scale_ptr(k_scale, fp8, "k_scale"), _scale_ptr(v_scale, fp8, "v_scale"), stream)
+        rows, hq, hkv, d, page, code, _scale_ptr(k_scale, fp8, "k_scale") or 0, _scale_ptr(v_scale, fp8, "v_scale") or 0,
+        scale), stream)
     if rc:
         _lib.check("hkb_paged_sparse_decode", rc)
     return out

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 from typing import Optional
@@ -97,18 +98,12 @@ SIGNATURES = {
     "hkb_prefill_tc_error": (c_int, [c_int]),
     "hkb_merge": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
                           c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
-    "hkb_advance_tables": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_void_p,
-                                   c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
-    "hkb_page_bounds": (c_int, [c_void_p, c_int64, c_int64, c_int64, CacheT, c_void_p, c_int64, c_int, c_void_p, c_void_p,
-                                c_int, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
-    "hkb_page_scores": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
-                                c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
-                                c_void_p, c_void_p]),
-    "hkb_select_pages": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int,
-                                 c_int, c_int, c_int, c_int, c_void_p]),
-    "hkb_paged_sparse_decode": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, CacheT, CacheT,
-                                        c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int64, c_int,
-                                        c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_void_p]),
+    # their arguments are structs of 64-bit fields, packed by the formats below: bytes, the stream
+    "hkb_advance_tables": (c_int, [c_char_p, c_void_p]),
+    "hkb_page_bounds": (c_int, [c_char_p, c_void_p]),
+    "hkb_page_scores": (c_int, [c_char_p, c_void_p]),
+    "hkb_select_pages": (c_int, [c_char_p, c_void_p]),
+    "hkb_paged_sparse_decode": (c_int, [c_char_p, c_void_p]),
     "hkb_walk_uses_mma": (c_int, [c_int, c_int]),
     "hkb_plan_splits": (c_int, [c_int, c_int, c_int, c_int]),
     "hkb_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
@@ -119,6 +114,14 @@ SIGNATURES = {
     "hkb_last_cuda_error": (c_int, []),
     "hkb_version": (c_int, []),
 }
+
+#: The argument structs of include/hkb.h whose fields are all eight bytes (pointers, int64_t, one double at the end):
+#: pack(fields in order) -> the bytes the call reads. A NULL pointer is 0.
+ADVANCE = struct.Struct("@15q").pack                # hkb_advance_t
+PAGE_BOUNDS = struct.Struct("@20q").pack            # hkb_page_bounds_t
+PAGE_SCORES = struct.Struct("@21qd").pack           # hkb_page_scores_t
+SELECT_PAGES = struct.Struct("@14q").pack           # hkb_select_pages_t
+SPARSE_DECODE = struct.Struct("@33qd").pack         # hkb_sparse_decode_t
 
 _LIB: Optional[ctypes.CDLL] = None
 

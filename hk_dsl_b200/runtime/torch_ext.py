@@ -15,6 +15,15 @@ names are registered on demand onto ONE runtime-parameterised C entry point:
     hk::paged_decode_fused_d{D}_s{S}(q, k_cache, v_cache, block_table, seq_lens, out!, o_part!, ml_part!)
     hk::paged_merge_d{D}_s{S}(seq_lens, out!, o_part, ml_part)
     hk::paged_prefill_d{D}_g{G}(q, k_cache, v_cache, block_table, seq_lens, q_start, tiles, out!)
+    hk::advance_tables(block_tables!, seq_lens!, new_tokens, free_pages!, free_count!, block_size, slot_mapping!, positions!,
+                       query_start_loc!, status!)
+    hk::update_page_bounds(bounds!, key_cache, block_tables, seq_lens, query_start_loc?, num_tokens)
+    hk::page_scores(scores!, query, bounds, block_tables, seq_lens, scale, block_size, kv_cache_dtype, k_scale?)
+    hk::select_pages(pages!, scores, seq_lens, block_size, first, last)
+    hk::paged_sparse_decode(out!, query, key_cache, value_cache, block_tables, seq_lens, pages, scale, kv_cache_dtype,
+                            k_scale?, v_scale?, out_lse!?)
+
+The last five (decode over selected pages, `hk_dsl_b200.ops.paged_sparse`) have no counterpart in hk-dsl.
 
 The split scratch (`o_part`, `ml_part`) is this build's: fp32 normalised partials and their
 natural-log lse (`hk_dsl_b200.ops.paged.fused_scratch`), caller-owned and allocated once.
@@ -27,7 +36,7 @@ from typing import Callable, Dict
 import torch
 
 from ..integration import engine
-from ..ops import paged
+from ..ops import paged, paged_sparse
 
 NS = "hk"
 _OPS: Dict[str, engine.Op] = {}
@@ -147,6 +156,45 @@ def prefill_op(head_dim: int, group: int) -> engine.Op:
     return _define(f"paged_prefill_d{head_dim}_g{group}",
                    "(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, Tensor q_start, "
                    "Tensor tiles, Tensor(a!) out) -> ()", impl)
+
+
+def _update_page_bounds(bounds, key_cache, block_tables, seq_lens, query_start_loc, num_tokens):
+    paged_sparse.update_page_bounds(bounds, key_cache, block_tables, seq_lens, query_start_loc, num_tokens=num_tokens)
+
+
+def _page_scores(scores, query, bounds, block_tables, seq_lens, scale, block_size, kv_cache_dtype, k_scale):
+    paged_sparse.page_scores(scores, query, bounds, block_tables, seq_lens, scale, block_size, kv_cache_dtype, k_scale)
+
+
+def _select_pages(pages, scores, seq_lens, block_size, first, last):
+    paged_sparse.select_pages(pages, scores, seq_lens, block_size, first=first, last=last)
+
+
+def _paged_sparse_decode(out, query, key_cache, value_cache, block_tables, seq_lens, pages, scale, kv_cache_dtype,
+                         k_scale, v_scale, out_lse):
+    paged_sparse.paged_sparse_decode(out, query, key_cache, value_cache, block_tables, seq_lens, pages, scale,
+                                     kv_cache_dtype, k_scale, v_scale, out_lse=out_lse)
+
+
+def sparse_ops() -> Dict[str, engine.Op]:
+    """The operators of a decode over selected pages by name, defined on the first call."""
+    return {name: _define(name, schema, impl) for name, schema, impl in (
+        ("advance_tables",
+         "(Tensor(a!) block_tables, Tensor(b!) seq_lens, Tensor new_tokens, Tensor(c!) free_pages, Tensor(d!) free_count, "
+         "int block_size, Tensor(e!) slot_mapping, Tensor(f!) positions, Tensor(g!) query_start_loc, Tensor(h!) status) "
+         "-> ()", paged_sparse.advance_tables),
+        ("update_page_bounds",
+         "(Tensor(a!) bounds, Tensor key_cache, Tensor block_tables, Tensor seq_lens, Tensor? query_start_loc, "
+         "int num_tokens) -> ()", _update_page_bounds),
+        ("page_scores",
+         "(Tensor(a!) scores, Tensor query, Tensor bounds, Tensor block_tables, Tensor seq_lens, float scale, "
+         "int block_size, str kv_cache_dtype, Tensor? k_scale) -> ()", _page_scores),
+        ("select_pages",
+         "(Tensor(a!) pages, Tensor scores, Tensor seq_lens, int block_size, int first, int last) -> ()", _select_pages),
+        ("paged_sparse_decode",
+         "(Tensor(a!) out, Tensor query, Tensor key_cache, Tensor value_cache, Tensor block_tables, Tensor seq_lens, "
+         "Tensor pages, float scale, str kv_cache_dtype, Tensor? k_scale, Tensor? v_scale, Tensor(b!)? out_lse) -> ()",
+         _paged_sparse_decode))}
 
 
 def launcher(kind: str, head_dim: int, splits: int) -> engine.Op:

@@ -452,6 +452,13 @@ int hkb_paged_decode_static(void* out, int64_t out_stride_tok, int64_t out_strid
                             int num_splits, void* stream);
 
 /*
+ * Decode over selected pages, and the page bookkeeping under it. These calls are made a handful a layer and take a few
+ * microseconds on the GPU, and they have many arguments, so each takes them in one struct (read before it returns) whose
+ * every field is eight bytes: a binder fills it as one array of 64-bit words. (From Python, 28 arguments by ctypes
+ * cost 2.6 us a call, the packed struct 0.6.) Counts and sizes must fit an int, except where a field says otherwise.
+ */
+
+/*
  * Block tables, slots and positions of a step from request lengths, on the device and in place. Request i of
  * num_reqs holds seq_lens[i] tokens (negative counts as 0) in pages of block_size and asks for new_tokens[i]
  * more; a negative value gives that many back from its end (rejected drafts; a whole length: a finished
@@ -474,11 +481,22 @@ int hkb_paged_decode_static(void* out, int64_t out_stride_tok, int64_t out_strid
 #define HKB_REQ_NO_PAGES 1    /* too few free pages */
 #define HKB_REQ_TABLE_FULL 2  /* more pages than the block table has columns, or more than 2^31 - 1 tokens */
 #define HKB_REQ_NO_ROWS 3     /* its rows end behind num_rows */
-int hkb_advance_tables(int32_t* block_table, int64_t table_stride, int max_pages, int32_t* seq_lens,
-                       const int32_t* new_tokens, int num_reqs, int block_size,
-                       int32_t* free_pages, int64_t free_capacity, int32_t* free_count,
-                       int64_t* slot_mapping, int64_t* positions, int64_t num_rows,
-                       int32_t* q_start, int32_t* status, void* stream);
+typedef struct {
+  int32_t* block_table;      /* (num_reqs, max_pages), table_stride elements a row */
+  int64_t table_stride, max_pages;
+  int32_t* seq_lens;
+  const int32_t* new_tokens;
+  int64_t num_reqs, block_size;
+  int32_t* free_pages;
+  int64_t free_capacity;
+  int32_t* free_count;
+  int64_t* slot_mapping;
+  int64_t* positions;
+  int64_t num_rows;          /* at most 2^30 */
+  int32_t* q_start;
+  int32_t* status;
+} hkb_advance_t;
+int hkb_advance_tables(const hkb_advance_t* args, void* stream);
 
 /*
  * Page summaries for a decode over selected pages: bounds[b, h, 0, :] and bounds[b, h, 1, :] become the least and
@@ -490,10 +508,17 @@ int hkb_advance_tables(int32_t* block_table, int64_t table_stride, int max_pages
  * [0, min(bounds_blocks, k_cache.num_blocks)) are skipped. num_tokens: an upper bound of q_start[num_seqs], which
  * must not be below it. block_size is any positive number.
  */
-int hkb_page_bounds(void* bounds, int64_t bounds_stride_block, int64_t bounds_stride_head, int64_t bounds_blocks,
-                    hkb_cache_t k_cache, const int32_t* block_table, int64_t table_stride, int max_pages,
-                    const int32_t* seq_lens, const int32_t* q_start, int num_seqs, int64_t num_tokens,
-                    int num_kv_heads, int head_dim, int block_size, int kv_dtype, void* stream);
+typedef struct {
+  void* bounds;
+  int64_t bounds_stride_block, bounds_stride_head, bounds_blocks;   /* bounds_blocks: any 64-bit count */
+  hkb_cache_t k_cache;
+  const int32_t* block_table;
+  int64_t table_stride, max_pages;
+  const int32_t* seq_lens;
+  const int32_t* q_start;    /* num_seqs + 1, or NULL */
+  int64_t num_seqs, num_tokens, num_kv_heads, head_dim, block_size, kv_dtype;
+} hkb_page_bounds_t;
+int hkb_page_bounds(const hkb_page_bounds_t* args, void* stream);
 
 /*
  * Page scores: scores[r, h, p] = scale * k_scale * max over the query heads g of kv head h of
@@ -503,12 +528,21 @@ int hkb_page_bounds(void* bounds, int64_t bounds_stride_block, int64_t bounds_st
  * the table. A NaN among a page's products makes its score NaN. q is bf16 (fp16 with HKB_KV_F16); scores fp32 with
  * contiguous columns; k_scale as in hkb_paged_decode.
  */
-int hkb_page_scores(float* scores, int64_t scores_stride_row, int64_t scores_stride_head, int num_columns,
-                    const void* q, int64_t q_stride_row, int64_t q_stride_head,
-                    const void* bounds, int64_t bounds_stride_block, int64_t bounds_stride_head, int64_t bounds_blocks,
-                    const int32_t* block_table, int64_t table_stride, const int32_t* seq_lens,
-                    int num_rows, int num_q_heads, int num_kv_heads, int head_dim, int block_size, float scale,
-                    int kv_dtype, const float* k_scale, void* stream);
+typedef struct {
+  float* scores;
+  int64_t scores_stride_row, scores_stride_head, num_columns;
+  const void* q;
+  int64_t q_stride_row, q_stride_head;
+  const void* bounds;
+  int64_t bounds_stride_block, bounds_stride_head, bounds_blocks;   /* bounds_blocks: any 64-bit count */
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* seq_lens;
+  int64_t num_rows, num_q_heads, num_kv_heads, head_dim, block_size, kv_dtype;
+  const float* k_scale;
+  double scale;
+} hkb_page_scores_t;
+int hkb_page_scores(const hkb_page_scores_t* args, void* stream);
 
 /*
  * The budget's best pages of every (row, kv head). Row r has n = min(ceil(seq_lens[r] / block_size), num_columns)
@@ -516,10 +550,15 @@ int hkb_page_scores(float* scores, int64_t scores_stride_row, int64_t scores_str
  * page, NaN above all numbers), min(n, budget) in all. pages[r, h, :] gets them in ascending order, -1 behind.
  * first + last <= budget. Columns at or past n are not read.
  */
-int hkb_select_pages(int32_t* pages, int64_t pages_stride_row, int64_t pages_stride_head, int budget,
-                     const float* scores, int64_t scores_stride_row, int64_t scores_stride_head, int num_columns,
-                     const int32_t* seq_lens, int num_rows, int num_kv_heads, int block_size, int first, int last,
-                     void* stream);
+typedef struct {
+  int32_t* pages;
+  int64_t pages_stride_row, pages_stride_head, budget;
+  const float* scores;
+  int64_t scores_stride_row, scores_stride_head, num_columns;
+  const int32_t* seq_lens;
+  int64_t num_rows, num_kv_heads, block_size, first, last;
+} hkb_select_pages_t;
+int hkb_select_pages(const hkb_select_pages_t* args, void* stream);
 
 /*
  * Decode attention over selected pages: hkb_paged_decode (one new token a row, the caches, dtypes, head sizes and
@@ -530,13 +569,24 @@ int hkb_select_pages(int32_t* pages, int64_t pages_stride_row, int64_t pages_str
  * the natural-log sum-exp of the scaled scores, so the answer can be merged with another (hkb_merge). scale and
  * k_scale must be positive. One launch, no scratch. out is 8-byte aligned, with strides that are multiples of 4.
  */
-int hkb_paged_sparse_decode(void* out, int64_t out_stride_tok, int64_t out_stride_head, float* out_lse,
-                            const void* q, int64_t q_stride_tok, int64_t q_stride_head,
-                            hkb_cache_t k_cache, hkb_cache_t v_cache,
-                            const int32_t* block_table, int64_t table_stride, int max_pages, const int32_t* seq_lens,
-                            const int32_t* pages, int64_t pages_stride_row, int64_t pages_stride_head, int budget,
-                            int num_rows, int num_q_heads, int num_kv_heads, int head_dim, int block_size, float scale,
-                            int kv_dtype, const float* k_scale, const float* v_scale, void* stream);
+typedef struct {
+  void* out;
+  int64_t out_stride_tok, out_stride_head;
+  float* out_lse;            /* or NULL */
+  const void* q;
+  int64_t q_stride_tok, q_stride_head;
+  hkb_cache_t k_cache, v_cache;
+  const int32_t* block_table;
+  int64_t table_stride, max_pages;
+  const int32_t* seq_lens;
+  const int32_t* pages;
+  int64_t pages_stride_row, pages_stride_head, budget;
+  int64_t num_rows, num_q_heads, num_kv_heads, head_dim, block_size, kv_dtype;
+  const float* k_scale;
+  const float* v_scale;
+  double scale;
+} hkb_sparse_decode_t;
+int hkb_paged_sparse_decode(const hkb_sparse_decode_t* args, void* stream);
 
 /*
  * Split planner: how many ways to cut the KV axis so that num_seqs*num_kv_heads

@@ -278,7 +278,7 @@ def _select(x, lens, page, budget, first, last):
     return out.cpu()
 
 
-@pytest.mark.parametrize("width", [1, 31, 64, 257, 1000, 2049, 9000])
+@pytest.mark.parametrize("width", [1, 31, 64, 257, 1000, 2000, 2049, 9000, 16385, 40000])
 @pytest.mark.parametrize("budget, first, last", [(1, 0, 0), (1, 1, 0), (5, 1, 4), (64, 1, 4), (300, 2, 0), (700, 0, 3)])
 def test_select_pages(width, budget, first, last):
     g = torch.Generator().manual_seed(width)
@@ -310,6 +310,18 @@ def test_select_pages_reads_no_column_behind_the_sequence_and_takes_strides():
     store = torch.full((3, 2, 11), 5, dtype=torch.int32, device="cuda")
     _ps().select_pages(store[:, :, :7], big[:, :, :50], torch.full((3,), 16 * 30, dtype=torch.int32).cuda(), 16, first=1, last=1)
     assert torch.equal(store[:, :, :7].cpu(), want) and (store[:, :, 7:] == 5).all()
+
+
+def test_select_pages_of_scores_that_share_a_histogram_bin():
+    """Keys in three far groups, the border inside one of them: every level of the digits is gone through."""
+    for width in (3000, 20000):
+        x = torch.empty(1, 1, width)
+        g = torch.Generator().manual_seed(width)
+        x[0, 0] = torch.where(torch.rand(width, generator=g) < 0.3, -1e30, 1.0)
+        near = torch.randint(0, 4, (width,), generator=g).float() * 2.0 ** -23 + 2.0
+        x[0, 0] = torch.where(torch.rand(width, generator=g) < 0.5, near, x[0, 0])
+        for budget in (1, 100, width // 4, width // 2, width - 1):
+            assert torch.equal(_select(x, [width * 16], 16, budget, 0, 0), orc.select_ref(x, [width * 16], 16, budget, 0, 0)), budget
 
 
 # ------------------------------------------------------------------------------ attention
@@ -584,6 +596,62 @@ def test_two_steps_at_once_on_two_streams():
     torch.cuda.synchronize()
     for s, (out, pages, slots) in zip(loops, alone):
         assert torch.equal(s.out, out) and torch.equal(s.pages, pages) and torch.equal(s.slots, slots)
+
+
+def test_fp8_bytes_in_uint8_storage():
+    c = _cache_case([200, 77], d=128, h_kv=2, group=4, kv="fp8", seed=31)
+    pages = _random_pages(c, 7)
+    b = _bounds_of(c)
+    got, lse = _attend(c, pages)
+    raw, rlse = _attend(c, pages, k=c["k"].view(torch.uint8), v=c["v"].view(torch.uint8))
+    assert torch.equal(got, raw) and torch.equal(lse, rlse)
+    s = [torch.empty(2, 2, c["table"].shape[1], device="cuda") for _ in range(2)]
+    for t, bb in zip(s, (b, b.view(torch.uint8))):
+        _ps().page_scores(t, c["q"].cuda(), bb.cuda(), c["table"].cuda(), _lens(c), c["scale"], 16, "fp8", c["ks"].cuda())
+    assert torch.equal(s[0], s[1])
+
+
+def test_answers_over_disjoint_pages_merge():
+    """Two selections' answers, folded by their sum-exps, are the answer over both."""
+    from hk_dsl_b200.ops import paged
+    c = _cache_case([700, 90, 0], d=128, h_kv=2, group=4, seed=41)
+    every = torch.arange(c["table"].shape[1], dtype=torch.int32).expand(3, 2, -1).contiguous()
+    parts = [_attend(c, every[:, :, i::2].contiguous()) for i in range(2)]
+    out = torch.empty(3, 8, 128, dtype=BF, device="cuda")
+    paged.merge_partials(out, torch.stack([p[0].float() for p in parts]), torch.stack([p[1] for p in parts]))
+    want, tol, _, _ = orc.sparse_ref(c["q"], c["k"], c["v"], c["table"], c["lens"], every, c["scale"])
+    # each part's own bounds (its rounding to bf16 among them), weighted, then one more rounding
+    part_tol = [orc.sparse_ref(c["q"], c["k"], c["v"], c["table"], c["lens"], every[:, :, i::2], c["scale"])[:3] for i in range(2)]
+    l = torch.stack([p[2] for p in part_tol])
+    w = torch.exp(l - torch.logsumexp(l, 0)).nan_to_num(0.0)
+    _hold(out, want, sum(w[i].unsqueeze(-1) * part_tol[i][1] for i in range(2)) * (1 + 2.0 ** -8) + want.abs() * 2.0 ** -8 + 2.0 ** -16)
+
+
+def test_a_step_without_new_rows_summarises_shortened_pages_again():
+    c = _cache_case([40, 21], d=64, h_kv=1, seed=51)
+    b = _bounds_of(c).cuda()
+    c["lens"] = [35, 5]
+    _ps().update_page_bounds(b, c["k"].cuda(), c["table"].cuda(), _lens(c), torch.zeros(3, dtype=torch.int32, device="cuda"), num_tokens=0)
+    want = orc.bounds_ref(_bounds_of(dict(c, lens=[40, 21])), c["k"], c["table"], [35, 5], [0, 0, 0])
+    assert _same(b, want)
+
+
+def test_the_torch_ops_are_the_calls():
+    from hk_dsl_b200.runtime import torch_ext
+    torch_ext.sparse_ops()
+    hk = torch.ops.hk
+    a, b = _Loop(5), _Loop(5)
+    for s in (a, b):
+        s.fill(0, STEPS[0])
+    a.step()
+    assert hk.advance_tables(b.table, b.lens, b.new, b.free, b.count, b.page, b.slots, b.pos, b.starts, b.status) is None
+    b.paged.reshape_and_cache(b.key, b.value, b.k, b.v, b.slots)
+    hk.update_page_bounds(b.bounds, b.k, b.table, b.lens, b.starts, b.rows)
+    hk.page_scores(b.scores, b.q, b.bounds, b.table, b.lens, b.scale, b.page, "auto", None)
+    hk.select_pages(b.pages, b.scores, b.lens, b.page, 1, 2)
+    hk.paged_sparse_decode(b.out, b.q, b.k, b.v, b.table, b.lens, b.pages, b.scale, "auto", None, None, b.lse)
+    for name in ("table", "lens", "free", "count", "slots", "pos", "starts", "status", "scores", "pages", "out", "lse"):
+        assert torch.equal(getattr(a, name), getattr(b, name)), name
 
 
 def test_the_same_call_twice_gives_the_same_bits():

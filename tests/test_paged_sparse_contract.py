@@ -1,6 +1,8 @@
 """Decode over selected pages: what the host refuses, before any launch and without a GPU, and the oracle's own rules."""
 
+import os
 import random
+import re
 
 import pytest
 import torch
@@ -96,50 +98,69 @@ def test_scores_select_and_bounds_refuse():
 
 def test_the_c_entries_refuse_before_any_launch():
     l = lib.load()
-    c = lib.CacheT(16, 2048, 128, 32768, 4)
 
     def adv(width=4, stride=4, lens=16, n=3, page=16, cap=8, count=16, slots=16, rows=5, starts=16):
-        return l.hkb_advance_tables(16, stride, width, lens, 16, n, page, 16, cap, count, slots, 16, rows, starts, 16, None)
+        return l.hkb_advance_tables(lib.ADVANCE(16, stride, width, lens, 16, n, page, 16, cap, count, slots, 16, rows, starts, 16), None)
 
-    assert adv(n=-1) == adv(rows=-1) == adv(cap=-1) == adv(cap=2 ** 31) == -9
+    assert adv(n=-1) == adv(rows=-1) == adv(cap=-1) == adv(cap=2 ** 31) == adv(width=2 ** 31) == adv(rows=2 ** 31) == -9
     assert adv(page=0) == -3 and adv(stride=3) == -6
-    assert adv(lens=None) == adv(count=None) == adv(slots=None) == adv(starts=None) == -1
+    assert adv(lens=0) == adv(count=0) == adv(slots=0) == adv(starts=0) == -1
 
-    def bnd(b=16, sb=256, cache=c, n=2, tok=4, hkv=1, d=128, page=16, dt=0, starts=None):
-        return l.hkb_page_bounds(b, sb, 256, 4, cache, 16, 4, 4, 16, starts, n, tok, hkv, d, page, dt, None)
+    def bnd(b=16, sb=256, sk=128, n=2, tok=4, hkv=1, d=128, page=16, dt=0, starts=0):
+        return l.hkb_page_bounds(lib.PAGE_BOUNDS(b, sb, 256, 4, 16, 2048, sk, 32768, 4, 16, 4, 4, 16, starts, n, tok, hkv, d, page, dt), None)
 
-    assert bnd(n=0) == 0 and bnd(starts=16, tok=0) == 0
-    assert bnd(n=-1) == bnd(hkv=0) == bnd(tok=-1) == -9 and bnd(b=None) == -1
+    assert bnd(n=0) == 0
+    assert bnd(n=-1) == bnd(hkv=0) == bnd(tok=-1) == bnd(n=2 ** 31) == -9 and bnd(b=0) == -1
     assert bnd(d=96) == -2 and bnd(page=0) == -3 and bnd(dt=7) == -5
-    assert bnd(sb=252) == -6 and bnd(b=24) == -7 and bnd(cache=lib.CacheT(16, 2048, 124, 32768, 4)) == -6
+    assert bnd(sb=252) == bnd(sk=124) == -6 and bnd(b=24) == -7
 
-    def sco(s=16, cols=8, q=16, qs=512, nb=4, rows=2, hq=4, hkv=2, d=128, page=16, dt=0, ks=None):
-        return l.hkb_page_scores(s, 16, 8, cols, q, qs, 128, 16, 512, 256, nb, 16, 8, 16, rows, hq, hkv, d, page, 0.1, dt, ks, None)
+    def sco(s=16, cols=8, q=16, qs=512, nb=4, rows=2, hq=4, hkv=2, d=128, page=16, dt=0, ks=0):
+        return l.hkb_page_scores(lib.PAGE_SCORES(s, 16, 8, cols, q, qs, 128, 16, 512, 256, nb, 16, 8, 16, rows, hq, hkv, d, page,
+                                                 dt, ks, 0.1), None)
 
     assert sco(rows=0) == 0 and sco(cols=0) == 0
-    assert sco(rows=-1) == sco(rows=65536) == sco(nb=0) == -9 and sco(s=None) == -1
+    assert sco(rows=-1) == sco(rows=65536) == sco(nb=0) == sco(cols=2 ** 31) == -9 and sco(s=0) == -1
     assert sco(d=96) == -2 and sco(page=0) == -3 and sco(hq=3) == sco(hq=34) == -4
     assert sco(dt=3) == -5 and sco(dt=1) == -10 and sco(qs=508) == -6 and sco(q=8) == sco(s=18) == -7
 
-    def sel(p=16, budget=8, s=16, cols=20, rows=2, page=16, first=1, last=4):
-        return l.hkb_select_pages(p, 16, 8, budget, s, 40, 20, cols, 16, rows, 2, page, first, last, None)
+    def sel(p=16, budget=8, s=16, cols=20, rows=2, hkv=2, page=16, first=1, last=4):
+        return l.hkb_select_pages(lib.SELECT_PAGES(p, 16, 8, budget, s, 40, 20, cols, 16, rows, hkv, page, first, last), None)
 
     assert sel(rows=0) == 0 and sel(budget=0, first=0, last=0) == 0
-    assert sel(rows=-1) == sel(budget=4) == sel(first=-1) == -9 and sel(p=None) == sel(s=None) == -1
+    assert sel(rows=-1) == sel(budget=4) == sel(first=-1) == sel(rows=2 ** 30) == sel(hkv=65536) == -9 and sel(p=0) == sel(s=0) == -1
     assert sel(page=0) == -3 and sel(p=18) == -7
 
-    def att(out=16, os=512, lse=None, q=16, cache=c, table=16, pages=16, budget=4, rows=2, hq=4, hkv=2, d=128, page=16,
-            dt=0, ks=None):
-        return l.hkb_paged_sparse_decode(out, os, 128, lse, q, 512, 128, cache, cache, table, 8, 8, 16, pages, 8, 4, budget,
-                                         rows, hq, hkv, d, page, 0.1, dt, ks, None, None)
+    def att(out=16, os=512, lse=0, q=16, sk=128, nb=4, table=16, pages=16, budget=4, rows=2, hq=4, hkv=2, d=128, page=16, dt=0, ks=0):
+        return l.hkb_paged_sparse_decode(lib.SPARSE_DECODE(
+            out, os, 128, lse, q, 512, 128, 16, 2048, sk, 32768, nb, 16, 2048, 128, 32768, 4, table, 8, 8, 16, pages, 8, 4, budget,
+            rows, hq, hkv, d, page, dt, ks, 0, 0.1), None)
 
     assert att(rows=0) == 0
-    assert att(rows=-1) == att(rows=65536) == att(budget=-1) == -9 and att(budget=2 ** 31 - 1, page=32) == -9
-    assert att(out=None) == att(q=None) == att(table=None) == att(pages=None) == -1
+    assert att(rows=-1) == att(rows=65536) == att(budget=-1) == att(nb=0) == -9 and att(budget=2 ** 31 - 1, page=32) == -9
+    assert att(out=0) == att(q=0) == att(table=0) == att(pages=0) == -1
     assert att(d=96) == -2 and att(page=24) == -3 and att(hq=3) == att(hq=34) == -4 and att(dt=9) == -5
     assert att(dt=1) == att(dt=1, ks=16) == -10
-    assert att(os=510) == -6 and att(out=20) == att(lse=18) == att(q=8) == -7
-    assert att(cache=lib.CacheT(16, 2048, 124, 32768, 4)) == -6 and att(cache=lib.CacheT(16, 2048, 128, 32768, 0)) == -9
+    assert att(os=510) == att(sk=124) == -6 and att(out=20) == att(lse=18) == att(q=8) == -7
+    for fn in ("hkb_advance_tables", "hkb_page_bounds", "hkb_page_scores", "hkb_select_pages", "hkb_paged_sparse_decode"):
+        assert getattr(l, fn)(None, None) == -1
+
+
+def test_the_argument_structs_are_packed_as_the_header_declares_them():
+    """One 64-bit word a field, in the header's order; hkb_cache_t is five words."""
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "hkb.h")).read()
+    for struct, pack in (("hkb_advance_t", lib.ADVANCE), ("hkb_page_bounds_t", lib.PAGE_BOUNDS),
+                         ("hkb_page_scores_t", lib.PAGE_SCORES), ("hkb_select_pages_t", lib.SELECT_PAGES),
+                         ("hkb_sparse_decode_t", lib.SPARSE_DECODE)):
+        body = re.search(r"typedef struct \{([^}]*)\} " + struct, text).group(1)
+        body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+        words, doubles = 0, []
+        for decl in filter(None, (d.strip() for d in body.split(";"))):
+            each = 5 if decl.startswith("hkb_cache_t") else 1
+            assert each == 5 or "*" in decl or decl.startswith(("int64_t", "double")), decl
+            doubles += [decl.startswith("double")] * (each * (decl.count(",") + 1))
+            words = len(doubles)
+        assert len(pack(*[0.0 if d else 0 for d in doubles])) == 8 * words, struct
+        assert not any(doubles[:-1])
 
 
 def test_the_oracles_tables_keep_every_page():
