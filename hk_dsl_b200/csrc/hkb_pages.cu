@@ -755,41 +755,56 @@ __global__ void __launch_bounds__(SELECT_WARPS * 32) select_warp_kernel(const Se
 }
 
 // Inclusive sum over the CTA's threads; `sums` is one value a warp, free to be written (a barrier behind its last read).
-template <int THREADS>
-__device__ __forceinline__ uint64_t select_scan(uint64_t v, uint64_t* sums, uint64_t& total) {
+template <int THREADS, class T>
+__device__ __forceinline__ T select_scan(T v, T* sums, T& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) {
-    const uint64_t y = __shfl_up_sync(0xffffffffu, v, x);
+    const T y = __shfl_up_sync(0xffffffffu, v, x);
     if (lane >= x) v += y;
   }
   if (lane == 31) sums[warp] = v;
   __syncthreads();
-  uint64_t w = lane < THREADS / 32 ? sums[lane] : 0;
-  const uint64_t own = w;
+  T w = lane < THREADS / 32 ? sums[lane] : 0;
+  const T own = w;
 #pragma unroll
-  for (int x = 1; x < 32; x <<= 1) {
-    const uint64_t y = __shfl_up_sync(0xffffffffu, w, x);
+  for (int x = 1; x < THREADS / 32; x <<= 1) {
+    const T y = __shfl_up_sync(0xffffffffu, w, x);
     if (lane >= x) w += y;
   }
-  total = __shfl_sync(0xffffffffu, w, 31);
+  total = __shfl_sync(0xffffffffu, w, THREADS / 32 - 1);
   return v + __shfl_sync(0xffffffffu, w - own, warp);
 }
 
 // RESIDENT: THREADS x EACH covers the row; otherwise the keys are read again for every pass, THREADS x EACH at a time.
 template <int THREADS, int EACH, bool RESIDENT>
 __global__ void __launch_bounds__(THREADS) select_kernel(const SelectArgs a) {
+  constexpr int SPAN = THREADS * EACH;
   __shared__ int hist[SELECT_BINS];
   __shared__ uint32_t ends[2][THREADS / 32];
-  __shared__ uint64_t sums[2][THREADS / 32];
+  __shared__ int sums[2][THREADS / 32];
+  __shared__ uint64_t places[2][THREADS / 32];
+  // of every 32 consecutive pages: which lie above the border, which on it, and how many do before them
+  constexpr int WORDS = SPAN / 32;
+  __shared__ uint32_t above_bits[WORDS], tie_bits[WORDS];
+  __shared__ uint64_t before[WORDS];
   __shared__ int s_bin, s_above, s_in;
-  constexpr int MINE = SELECT_BINS / THREADS, SPAN = THREADS * EACH;
+  constexpr int MINE = SELECT_BINS / THREADS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int head = blockIdx.y, row = blockIdx.x;
-  const int len = max(__ldg(a.seq_lens + row), 0);
-  const int n = (int)min(((int64_t)len + a.page - 1) / a.page, (int64_t)a.columns);
   int* out = a.pages + (int64_t)row * a.p_stride_row + (int64_t)head * a.p_stride_head;
   const float* in = a.scores + (int64_t)row * a.s_stride_row + (int64_t)head * a.s_stride_head + a.first;
+  uint32_t key[EACH];
+  auto load = [&](int p0, int end) {              // every THREADS-th page a thread
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int p = p0 + e * THREADS + tid;
+      key[e] = p < end ? score_key(__ldg(in + p)) : 0u;
+    }
+  };
+  if (RESIDENT) load(0, a.columns - a.first);     // beside the length, not behind it; the columns past it are not used
+  const int len = max(__ldg(a.seq_lens + row), 0);
+  const int n = (int)min(((int64_t)len + a.page - 1) / a.page, (int64_t)a.columns);
   if (n <= a.budget) {
     for (int i = tid; i < a.budget; i += THREADS) out[i] = i < n ? i : -1;
     return;
@@ -802,22 +817,14 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectArgs a) {
   if (want == 0) return;
   out += a.first;
 
-  uint32_t key[EACH];
-  auto load = [&](int p0) {                       // consecutive pages a thread
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      const int p = p0 + tid * EACH + e;
-      key[e] = p < m ? score_key(__ldg(in + p)) : 0u;
-    }
-  };
 #pragma unroll
   for (int i = 0; i < MINE; ++i) hist[tid * MINE + i] = 0;
   uint32_t least = 0xffffffffu, most = 0u;
   for (int p0 = 0; p0 < m; p0 += SPAN) {
-    load(p0);
+    if (!RESIDENT) load(p0, m);
 #pragma unroll
     for (int e = 0; e < EACH; ++e)
-      if (p0 + tid * EACH + e < m) { least = min(least, key[e]); most = max(most, key[e]); }
+      if (p0 + e * THREADS + tid < m) { least = min(least, key[e]); most = max(most, key[e]); }
   }
   least = __reduce_min_sync(0xffffffffu, least);
   most = __reduce_max_sync(0xffffffffu, most);
@@ -832,11 +839,11 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectArgs a) {
   bool whole = false;                             // all undecided keys are taken
   while (shift < 32) {
     for (int p0 = 0; p0 < m; p0 += SPAN) {
-      if (!RESIDENT) load(p0);
+      if (!RESIDENT) load(p0, m);
 #pragma unroll
       for (int e = 0; e < EACH; ++e) {
         const uint32_t x = key[e] - base;         // a key below base wraps to a great x
-        if (p0 + tid * EACH + e < m && key[e] >= base && (x >> (31 - shift)) <= 1u)
+        if (p0 + e * THREADS + tid < m && key[e] >= base && (x >> (31 - shift)) <= 1u)
           atomicAdd(&hist[(x << shift) >> (32 - SELECT_BITS)], 1);
       }
     }
@@ -849,8 +856,8 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectArgs a) {
       hist[SELECT_BINS - 1 - tid * MINE - i] = 0;
       mine += bins[i];
     }
-    uint64_t total;
-    int above = (int)select_scan<THREADS>((uint64_t)mine, sums[which], total) - mine;
+    int total;
+    int above = select_scan<THREADS>(mine, sums[which], total) - mine;
     which ^= 1;
     if (above < want && above + mine >= want) {   // one thread
       int i = 0;
@@ -871,29 +878,33 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectArgs a) {
   }
   // Taken: keys above `base`; of those equal to it the first `want` -- or all from it on, where `whole`.
   uint64_t done = 0;                              // keys above in the upper half, ties in the lower
+  const unsigned below = (1u << lane) - 1u;
+  static_assert(WORDS <= THREADS, "a word a thread");
   for (int p0 = 0; p0 < m; p0 += SPAN) {
-    if (!RESIDENT) load(p0);
-    uint64_t mine = 0;
+    if (!RESIDENT) load(p0, m);
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-      if (p0 + tid * EACH + e >= m) continue;
-      if (whole ? key[e] >= base : key[e] > base) mine += 1ull << 32;
-      else if (!whole && key[e] == base) mine += 1;
+      const bool in_row = p0 + e * THREADS + tid < m;
+      const uint32_t up = __ballot_sync(0xffffffffu, in_row && (whole ? key[e] >= base : key[e] > base));
+      const uint32_t tie = __ballot_sync(0xffffffffu, in_row && !whole && key[e] == base);
+      if (lane == 0) { above_bits[e * (THREADS / 32) + warp] = up; tie_bits[e * (THREADS / 32) + warp] = tie; }
     }
+    __syncthreads();
+    const uint64_t mine = tid < WORDS ? (uint64_t)__popc(above_bits[tid]) << 32 | __popc(tie_bits[tid]) : 0;
     uint64_t total;
-    const uint64_t incl = done + select_scan<THREADS>(mine, sums[which], total);
+    const uint64_t incl = done + select_scan<THREADS>(mine, places[which], total);
+    if (tid < WORDS) before[tid] = incl - mine;
+    __syncthreads();
     which ^= 1;
     done += total;
-    int at = (int)((incl - mine) >> 32), ties = (int)(uint32_t)(incl - mine);
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-      const int p = p0 + tid * EACH + e;
-      if (p >= m) continue;
-      const bool tie = !whole && key[e] == base;
-      if ((whole ? key[e] >= base : key[e] > base) || (tie && ties < want)) out[at + min(ties, want)] = a.first + p;
-      if (tie) ++ties;
-      else if (whole ? key[e] >= base : key[e] > base) ++at;
+      const int w = e * (THREADS / 32) + warp;
+      const uint32_t up = above_bits[w], tie = tie_bits[w];
+      const int at = (int)(before[w] >> 32) + __popc(up & below), ties = (int)(uint32_t)before[w] + __popc(tie & below);
+      if ((up >> lane & 1) || ((tie >> lane & 1) && ties < want)) out[at + min(ties, want)] = a.first + p0 + e * THREADS + tid;
     }
+    if (!RESIDENT) __syncthreads();               // the words are written again
   }
 }
 

@@ -5,8 +5,9 @@
 // waited for. So a score is added up in two chains of products, and the maximum over a tile is not taken at all where
 // it is not needed: a lane compares its own scores with the softmax reference, and only if one of the warp's exceeds it
 // by 2^8 (the first tile, and rarely after) are maxima exchanged and the accumulators rescaled. A tile then takes a warp
-// alone 0.52 us instead of 0.59 (the rest is the mma pipe of its quarter of the SM: two tiles a step, twice the
-// independent work, took the same time a tile and more shared memory).
+// alone 0.52 us instead of 0.59; what is left is the issue of its instructions one after another (the tensor pipe is
+// 16 % busy at twelve warps an SM). Two tiles a step took 0.48 us each and twice the shared memory: 16 x 8 items of 256
+// pages 61 against 67 us on a CTA each, but 64 x 8 of 64 pages 48.3 against 45.4, where the rings are what is short.
 #pragma once
 
 #include "hkb_walk_mma.cuh"
