@@ -1,4 +1,4 @@
-// Thread-block clusters: rank, barrier, a peer's shared memory, and the launch.
+// Thread-block clusters (rank, barrier, a peer's shared memory), launches that follow closely on one another.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -50,20 +50,29 @@ inline bool ints(std::initializer_list<int64_t> values) {
   return true;
 }
 
-// One argument struct, `cluster` CTAs of grid.x a cluster (1: an ordinary launch; past 8, the portable size,
-// the kernel has to be allowed to).
-inline int launch_cluster(const void* kernel, dim3 grid, int threads, int cluster, int smem_bytes, const void* args, cudaStream_t st) {
+// The calls of a decode step are short kernels that each read what the one before wrote. They are launched with
+// programmatic stream serialisation: a kernel's CTAs may take their places while the kernel before still runs. Every
+// kernel launched so begins with `after_the_last`, which waits until everything before it is complete and its writes are
+// seen (nothing is read or written in front of it), and calls `let_the_next` where the next one's CTAs may come in.
+__device__ __forceinline__ void after_the_last() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+__device__ __forceinline__ void let_the_next() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+
+// One argument struct; `cluster` CTAs of grid.x a cluster (1: none; past 8, the portable size, the kernel has to be
+// allowed to).
+inline int launch(const void* kernel, dim3 grid, int threads, int cluster, int smem_bytes, const void* args, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem_bytes;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   void* params[1] = {const_cast<void*>(args)};
   cudaError_t e = cudaLaunchKernelExC(&cfg, kernel, params);
   if (e == cudaSuccess) e = cudaGetLastError();

@@ -166,6 +166,8 @@ __device__ __forceinline__ int range_of_warp(const int* ends, int n, int x, int 
 template <int WARPS, int EACH>
 __global__ void __launch_bounds__(WARPS * 32) advance_kernel(const AdvanceArgs a) {
   __shared__ AdvChunk<WARPS, EACH> c;
+  after_the_last();
+  let_the_next();
   constexpr int THREADS = WARPS * 32, CHUNK = THREADS * EACH;
   const int tid = threadIdx.x, lane = tid & 31;
   const int ctas = cluster_size(), rank = cluster_rank();
@@ -348,6 +350,8 @@ __global__ void __launch_bounds__(BOUNDS_WARPS * 32) bounds_kernel(const BoundsA
   constexpr int REGS = FP8 ? 8 : 4;               // pairs a 16-byte chunk holds
   constexpr int RPI = 32 / CPR, UNROLL = 8;
   constexpr int STEP = RPI * UNROLL * (SHARE ? BOUNDS_WARPS : 1);
+  after_the_last();
+  let_the_next();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t unit = SHARE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * BOUNDS_WARPS + warp;
   const int item = (int)(unit / a.num_kv_heads), head = (int)(unit % a.num_kv_heads);
@@ -499,6 +503,8 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32) scores_kernel(const ScoreArg
   constexpr int MPC = EPC / 4;                 // mma a chunk feeds
   constexpr int CHAINS = NT == 1 ? 4 : 2;
   using Ring = ScoreRing<D, FP8>;
+  after_the_last();
+  let_the_next();
   extern __shared__ __align__(128) uint8_t hkb_smem[];
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int head = blockIdx.y, row = blockIdx.z;
@@ -672,6 +678,7 @@ struct SelectArgs {
   int columns;
   const int* seq_lens;
   int page, first, last;
+  int num_kv_heads, items;         // items: rows x kv heads
 };
 
 __device__ __forceinline__ uint32_t score_key(float x) {
@@ -684,11 +691,13 @@ __device__ __forceinline__ uint32_t score_key(float x) {
 constexpr int SELECT_WARPS = 4;
 
 template <int EACH>
-__global__ void __launch_bounds__(SELECT_WARPS * 32) select_warp_kernel(const SelectArgs a, int num_kv_heads, int64_t items) {
+__global__ void __launch_bounds__(SELECT_WARPS * 32) select_warp_kernel(const SelectArgs a) {
+  after_the_last();
+  let_the_next();
   const int lane = threadIdx.x & 31;
   const int64_t item = (int64_t)blockIdx.x * SELECT_WARPS + (threadIdx.x >> 5);
-  if (item >= items) return;
-  const int64_t row = item / num_kv_heads, head = item - row * num_kv_heads;
+  if (item >= a.items) return;
+  const int64_t row = item / a.num_kv_heads, head = item - row * a.num_kv_heads;
   const int len = max(__ldg(a.seq_lens + row), 0);
   int* out = a.pages + row * a.p_stride_row + head * a.p_stride_head;
   const float* in = a.scores + row * a.s_stride_row + head * a.s_stride_head;
@@ -790,6 +799,8 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectArgs a) {
   __shared__ uint64_t before[WORDS];
   __shared__ int s_bin, s_above, s_in;
   constexpr int MINE = SELECT_BINS / THREADS;
+  after_the_last();
+  let_the_next();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int head = blockIdx.y, row = blockIdx.x;
   int* out = a.pages + (int64_t)row * a.p_stride_row + (int64_t)head * a.p_stride_head;
@@ -908,14 +919,6 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectArgs a) {
   }
 }
 
-template <class F>
-static int launched(F&& launch) {
-  launch();
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) { hkb_tls_cuda_error = (int)e; return HKB_ERR_CUDA; }
-  return HKB_OK;
-}
-
 // More than 48 KB of dynamic shared memory, or a cluster past the portable size, is asked for once a device.
 template <class K>
 static cudaError_t arm(K kernel, cudaFuncAttribute attribute, int value, bool (&armed)[64]) {
@@ -934,7 +937,7 @@ static int launch_scores(const ScoreArgs& a, dim3 grid, cudaStream_t st) {
   static bool armed[64] = {};
   constexpr int smem = ScoreRing<D, KIND == HKB_KV_FP8_E4M3>::BYTES;
   if (arm(scores_kernel<KIND, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem, armed) != cudaSuccess) return HKB_ERR_CUDA;
-  return launched([&] { scores_kernel<KIND, D, NT><<<grid, SCORE_WARPS * 32, smem, st>>>(a); });
+  return launch((const void*)scores_kernel<KIND, D, NT>, grid, SCORE_WARPS * 32, 1, smem, &a, st);
 }
 
 static int advance_tables(int32_t* block_table, int64_t table_stride, int max_pages, int32_t* seq_lens,
@@ -964,9 +967,9 @@ static int advance_tables(int32_t* block_table, int64_t table_stride, int max_pa
     auto kernel = advance_kernel<32, 2>;
     static bool armed[64] = {};
     if (arm(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1, armed) != cudaSuccess) return HKB_ERR_CUDA;
-    return launch_cluster((const void*)kernel, dim3(16), 1024, 16, 0, &a, (cudaStream_t)stream);
+    return launch((const void*)kernel, dim3(16), 1024, 16, 0, &a, (cudaStream_t)stream);
   }
-  return launch_cluster((const void*)advance_kernel<8, 2>, dim3(1), 256, 1, 0, &a, (cudaStream_t)stream);
+  return launch((const void*)advance_kernel<8, 2>, dim3(1), 256, 1, 0, &a, (cudaStream_t)stream);
 }
 
 static int page_bounds(void* bounds, int64_t bounds_stride_block, int64_t bounds_stride_head, int64_t bounds_blocks,
@@ -995,18 +998,16 @@ static int page_bounds(void* bounds, int64_t bounds_stride_block, int64_t bounds
   a.table = block_table; a.table_stride = table_stride; a.max_pages = max_pages;
   a.seq_lens = seq_lens; a.q_start = q_start; a.num_seqs = num_seqs; a.num_kv_heads = num_kv_heads; a.page = block_size;
   a.items = (int)items;
-  cudaStream_t st = (cudaStream_t)stream;
-  return launched([&] {
 #define HKB_BOUNDS(KIND, CPR_) \
   if (kv_dtype == KIND && head_dim * es == CPR_ * 16) { \
-    if (share) bounds_kernel<KIND, CPR_, true><<<(unsigned)ctas, BOUNDS_WARPS * 32, 0, st>>>(a); \
-    else bounds_kernel<KIND, CPR_, false><<<(unsigned)ctas, BOUNDS_WARPS * 32, 0, st>>>(a); \
+    const void* kernel = share ? (const void*)bounds_kernel<KIND, CPR_, true> : (const void*)bounds_kernel<KIND, CPR_, false>; \
+    return launch(kernel, dim3((unsigned)ctas), BOUNDS_WARPS * 32, 1, 0, &a, (cudaStream_t)stream); \
   }
-    HKB_BOUNDS(HKB_KV_BF16, 8) HKB_BOUNDS(HKB_KV_BF16, 16) HKB_BOUNDS(HKB_KV_BF16, 32)
-    HKB_BOUNDS(HKB_KV_F16, 8) HKB_BOUNDS(HKB_KV_F16, 16) HKB_BOUNDS(HKB_KV_F16, 32)
-    HKB_BOUNDS(HKB_KV_FP8_E4M3, 4) HKB_BOUNDS(HKB_KV_FP8_E4M3, 8) HKB_BOUNDS(HKB_KV_FP8_E4M3, 16)
+  HKB_BOUNDS(HKB_KV_BF16, 8) HKB_BOUNDS(HKB_KV_BF16, 16) HKB_BOUNDS(HKB_KV_BF16, 32)
+  HKB_BOUNDS(HKB_KV_F16, 8) HKB_BOUNDS(HKB_KV_F16, 16) HKB_BOUNDS(HKB_KV_F16, 32)
+  HKB_BOUNDS(HKB_KV_FP8_E4M3, 4) HKB_BOUNDS(HKB_KV_FP8_E4M3, 8) HKB_BOUNDS(HKB_KV_FP8_E4M3, 16)
 #undef HKB_BOUNDS
-  });
+  return HKB_ERR_UNSUPPORTED;
 }
 
 static int page_scores(float* scores, int64_t scores_stride_row, int64_t scores_stride_head, int num_columns,
@@ -1071,18 +1072,18 @@ static int select_pages(int32_t* pages, int64_t pages_stride_row, int64_t pages_
   a.seq_lens = seq_lens; a.page = block_size; a.first = first; a.last = last;
   const int64_t items = (int64_t)num_rows * num_kv_heads;
   if (items > 0x7fffffff) return HKB_ERR_SIZE;
-  const dim3 grid(num_rows, num_kv_heads);
+  a.num_kv_heads = num_kv_heads; a.items = (int)items;
   cudaStream_t st = (cudaStream_t)stream;
-  return launched([&] {
-    const unsigned ctas = (unsigned)((items + SELECT_WARPS - 1) / SELECT_WARPS);
-    if (num_columns <= 256) select_warp_kernel<8><<<ctas, SELECT_WARPS * 32, 0, st>>>(a, num_kv_heads, items);
-    else if (num_columns <= 512) select_warp_kernel<16><<<ctas, SELECT_WARPS * 32, 0, st>>>(a, num_kv_heads, items);
-    else if (num_columns <= 1024) select_warp_kernel<32><<<ctas, SELECT_WARPS * 32, 0, st>>>(a, num_kv_heads, items);
-    else if (num_columns <= 2048) select_kernel<256, 8, true><<<grid, 256, 0, st>>>(a);
-    else if (num_columns <= 8192) select_kernel<1024, 8, true><<<grid, 1024, 0, st>>>(a);
-    else if (num_columns <= 16384) select_kernel<1024, 16, true><<<grid, 1024, 0, st>>>(a);
-    else select_kernel<1024, 16, false><<<grid, 1024, 0, st>>>(a);
-  });
+  if (num_columns <= 1024) {       // 32 keys a lane at most
+    const void* kernel = num_columns <= 256 ? (const void*)select_warp_kernel<8>
+                         : num_columns <= 512 ? (const void*)select_warp_kernel<16> : (const void*)select_warp_kernel<32>;
+    return launch(kernel, dim3((unsigned)((items + SELECT_WARPS - 1) / SELECT_WARPS)), SELECT_WARPS * 32, 1, 0, &a, st);
+  }
+  const dim3 grid(num_rows, num_kv_heads);
+  if (num_columns <= 2048) return launch((const void*)select_kernel<256, 8, true>, grid, 256, 1, 0, &a, st);
+  const void* kernel = num_columns <= 8192 ? (const void*)select_kernel<1024, 8, true>
+                       : num_columns <= 16384 ? (const void*)select_kernel<1024, 16, true> : (const void*)select_kernel<1024, 16, false>;
+  return launch(kernel, grid, 1024, 1, 0, &a, st);
 }
 
 }  // namespace hkb
