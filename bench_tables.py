@@ -9,6 +9,7 @@ here is part of the bench line.
     python bench_tables.py --prefill-trace [--case 1x0+8192]
                                          where the tensor-memory prefill kernel's cycles go, by role
     python bench_tables.py --attrib      the decode walk with one stage left out: what each stage costs
+    python bench_tables.py --sparse      a decode step over selected pages, call by call, beside the dense one
 """
 
 from __future__ import annotations
@@ -575,6 +576,75 @@ def layouts_table(only: str = ""):
     return 0 if same else 1
 
 
+def sparse_table():
+    """One layer's decode step over selected pages (hk_dsl_b200.ops.paged_sparse) -- the newest pages' summaries, scores,
+    selection, attention -- beside the dense walk and merge over the same caches: us from CUDA graphs whose calls rotate
+    through enough caches to read past L2 (>= 256 MB of summaries and selected pages a cycle where they fit), median of 7."""
+    import torch
+
+    from hk_dsl_b200 import workloads as W
+    from hk_dsl_b200.ops import paged, paged_sparse as ps
+
+    dev = torch.device("cuda", 0)
+    torch.cuda.set_device(dev)
+
+    def timed(call, layers):
+        for l in range(layers):
+            call(l)
+        torch.cuda.synchronize()
+        reps = max(1, 32 // layers)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for _ in range(reps):
+                for l in range(layers):
+                    call(l)
+        g.replay()
+        torch.cuda.synchronize()
+        times = []
+        for _ in range(7):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            g.replay()
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b) * 1e3 / (reps * layers))
+        return round(statistics.median(times), 2)
+
+    for reqs, hq, hkv, ctx, kv, budget in ((1, 32, 8, 32768, "auto", 128), (16, 32, 8, 8192, "auto", 64), (64, 32, 8, 8192, "auto", 64),
+                                           (128, 32, 8, 4096, "fp8", 64), (2, 64, 8, 131072, "auto", 256),
+                                           (2, 64, 8, 131072, "auto", 512), (2, 64, 8, 131072, "fp8", 256)):
+        spec = W.Spec("sparse", reqs, hq, hkv, kv_cache_dtype=kv, dist="fixed", lo=ctx, hi=ctx)
+        cache = spec.kv_bytes([ctx] * reqs)
+        touched = cache // 32 + min(cache, reqs * hkv * budget * 16 * 128 * 2 * spec.kv_elt)
+        layers = max(2, min(-(-(256 << 20) // touched), (24 << 30) // cache, 64))
+        st = W.build_step(spec, dev, layers=layers, seed=1)
+        n, page, width = reqs, spec.block_size, st.block_table.shape[1]
+        bounds = [ps.page_bounds(k) for k in st.k_caches]
+        whole = torch.arange(n + 1, dtype=torch.int32, device=dev) * ctx
+        for b, k in zip(bounds, st.k_caches):
+            ps.update_page_bounds(b, k, st.block_table, st.seq_lens, whole, num_tokens=n * ctx)
+        scores = torch.empty(n, hkv, width, device=dev)
+        pages = torch.empty(n, hkv, budget, dtype=torch.int32, device=dev)
+        splits = paged.plan_splits(n, hkv, width, device=dev)
+        scratch = paged.split_scratch(n, hq, 128, splits, dev)
+        calls = {
+            "summaries": lambda l: ps.update_page_bounds(bounds[l], st.k_caches[l], st.block_table, st.seq_lens),
+            "scores": lambda l: ps.page_scores(scores, st.query, bounds[l], st.block_table, st.seq_lens, st.scale, page, kv, st.k_scale),
+            "selection": lambda l: ps.select_pages(pages, scores, st.seq_lens, page),
+            "attention": lambda l: ps.paged_sparse_decode(st.out, st.query, st.k_caches[l], st.v_caches[l], st.block_table,
+                                                          st.seq_lens, pages, st.scale, kv, st.k_scale, st.v_scale)}
+        row = {"requests": n, "q_heads": hq, "kv_heads": hkv, "context": ctx, "kv": kv, "budget_pages": budget, "layers_rotated": layers}
+        row["dense_us"] = timed(lambda l: paged.paged_attention_decode(
+            st.out, st.query, st.k_caches[l], st.v_caches[l], st.block_table, st.seq_lens, st.scale, kv, st.k_scale, st.v_scale,
+            num_splits=splits, scratch=scratch), layers)
+        row["sparse_step_us"] = timed(lambda l: [c(l) for c in calls.values()], layers)
+        row.update({f"{k}_us": timed(c, layers) for k, c in calls.items()})
+        print(json.dumps(row), flush=True)
+        del st, bounds
+        torch.cuda.empty_cache()
+    return 0
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--latency", action="store_true")
@@ -584,10 +654,13 @@ def main():
     ap.add_argument("--prefill-trace", action="store_true", help="cycles by role and phase of the tensor-memory prefill kernel")
     ap.add_argument("--attrib", action="store_true", help="the decode walk with one stage left out: what each stage costs")
     ap.add_argument("--kv", default="bf16", choices=["bf16", "fp8"], help="with --prefill-trace, or --prefill --case: the cache type")
+    ap.add_argument("--sparse", action="store_true", help="a decode step over selected pages, call by call, beside the dense one")
     ap.add_argument("--exchange", action="store_true", help="the KV-split exchange kernels on one GPU (one launch against two)")
     ap.add_argument("--shards", action="store_true", help="one rank's share of c2 over 1/2/4/8 GPUs, on one GPU: the step's fixed costs")
     ap.add_argument("--layouts", action="store_true", help="the decode over the usual and the x-split cache layout")
     args = ap.parse_args()
+    if args.sparse:
+        return sparse_table()
     if args.exchange:
         return exchange_table(args.case)
     if args.shards:

@@ -19,7 +19,9 @@ namespace hkb {
 // every CTA scans all requests (a chunk of CHUNK at a time: one trip to memory and one three-fold scan), then takes
 // its share of the tokens and pages; the in-place updates -- the stack's top, the lengths, the count -- come after a
 // cluster barrier, when every CTA has read what it needs of the old state. Deterministic: no atomics.
-// Bound: latency (the scan, then two dependent trips), then the stores of 16 bytes a token.
+// Bound: latency (the scan, then two dependent trips), then the stores of 16 bytes a token. Measured, us a call: 64
+// requests decoding 3.5 (one CTA of 256 threads), 2048 requests with 48 prompts of 2731 tokens 11.7 (a cluster of sixteen
+// CTAs of 1024 threads; of 512 threads 14.8).
 // ---------------------------------------------------------------------------------
 constexpr int ADV_BLOCKS = 2;                     // 32-token blocks a warp looks up at once
 
@@ -296,7 +298,9 @@ __global__ void __launch_bounds__(WARPS * 32) advance_kernel(const AdvanceArgs a
 // sequence's length. Values of the cache's own type, so nothing is rounded. A warp takes a (page, kv head) -- of
 // pages of more than 32 tokens the CTA's four warps share it, or a decode step's few large pages would each be one
 // warp's chain of trips to memory: its lanes hold 16-byte chunks of a row, 32 / chunks rows at a time, and fold them
-// with packed minima and maxima that keep a NaN. Bound: bytes (the keys once, two rows a page out).
+// with packed minima and maxima that keep a NaN. Bound: bytes (the keys once, two rows a page out). Measured at head size
+// 128, eight kv heads: 4 x 8192 new tokens 14.8 us = 5.1 TB/s; 64 decoding sequences 2.0 us, with pages of 256 tokens
+// 6.9 (15.0 with a warp a page).
 // ---------------------------------------------------------------------------------
 constexpr int BOUNDS_WARPS = 4;
 
@@ -460,7 +464,9 @@ __global__ void __launch_bounds__(BOUNDS_WARPS * 32) bounds_kernel(const BoundsA
 // so lane t of a quad takes eight (fp8: sixteen) consecutive ones and the query's fragments are dealt alike. Since a
 // lane then reads nothing that another one fetched, the copies run through a cp.async ring in which every lane has its
 // own 16-byte places: asynchronous and deep as a walk's ring, without a barrier or a swizzle.
-// Bound: bytes (a summary is 2 rows a page where the attention reads 2 rows a token).
+// Bound: bytes (a summary is 2 rows a page where the attention reads 2 rows a token). Measured: 2 x 8192 pages, eight kv
+// heads of eight query heads, 13.6 us = 4.9 TB/s (loads straight into registers, two tiles a warp: 14.7 to 16; rings in
+// CTAs of four warps instead of one: 17.0, one chain of products a score: 17.3); four sequences of up to 32 pages 1.9 us.
 // ---------------------------------------------------------------------------------
 constexpr int SCORE_WARPS = 1;
 template <int D, bool FP8>
@@ -1074,13 +1080,19 @@ static int select_pages(int32_t* pages, int64_t pages_stride_row, int64_t pages_
   if (items > 0x7fffffff) return HKB_ERR_SIZE;
   a.num_kv_heads = num_kv_heads; a.items = (int)items;
   cudaStream_t st = (cudaStream_t)stream;
-  if (num_columns <= 1024) {       // 32 keys a lane at most
+  int sms = hkb_sm_count(-1);
+  if (sms <= 0) sms = 148;
+  const dim3 grid(num_rows, num_kv_heads);
+  // A warp's steps cost a comparison a key it holds, a CTA's its barriers. Measured, us, (rows x kv heads) of 1000 columns:
+  // 8 of them a warp each 6.5, a CTA each 5.2; 64: 7.2, 5.3; 512: 7.6, 9.7; 4096: 18, 45. Of 500: 4.0, 4.3; 4.5, 4.8.
+  if (num_columns <= 512 || (num_columns <= 1024 && items > 2 * sms)) {
     const void* kernel = num_columns <= 256 ? (const void*)select_warp_kernel<8>
                          : num_columns <= 512 ? (const void*)select_warp_kernel<16> : (const void*)select_warp_kernel<32>;
     return launch(kernel, dim3((unsigned)((items + SELECT_WARPS - 1) / SELECT_WARPS)), SELECT_WARPS * 32, 1, 0, &a, st);
   }
-  const dim3 grid(num_rows, num_kv_heads);
-  if (num_columns <= 2048) return launch((const void*)select_kernel<256, 8, true>, grid, 256, 1, 0, &a, st);
+  // 2000 columns: 8 of them 5.1, 512 10.6 (1024 threads of two keys: 4.9, 16.9). 8000: 8.4 (512 threads of 16: 9.8).
+  if (num_columns <= 2048)
+    return launch(num_columns <= 1024 ? (const void*)select_kernel<256, 4, true> : (const void*)select_kernel<256, 8, true>, grid, 256, 1, 0, &a, st);
   const void* kernel = num_columns <= 8192 ? (const void*)select_kernel<1024, 8, true>
                        : num_columns <= 16384 ? (const void*)select_kernel<1024, 16, true> : (const void*)select_kernel<1024, 16, false>;
   return launch(kernel, grid, 1024, 1, 0, &a, st);
