@@ -57,9 +57,14 @@ inline bool ints(std::initializer_list<int64_t> values) {
 __device__ __forceinline__ void after_the_last() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 __device__ __forceinline__ void let_the_next() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
 
+// The percentage of an SM's memory that is shared memory. One split for a step's kernels: an SM that changes it empties
+// first, so a step that alternated kernels with and without rings lost the head start (2 requests x 131072 tokens, 256
+// pages: 41.2 against 36.2 us a step).
+constexpr int STEP_CARVEOUT = 100;
+
 // One argument struct; `cluster` CTAs of grid.x a cluster (1: none; past 8, the portable size, the kernel has to be
 // allowed to).
-inline int launch(const void* kernel, dim3 grid, int threads, int cluster, int smem_bytes, const void* args, cudaStream_t st) {
+inline int launch(const void* kernel, dim3 grid, int threads, int cluster, int smem_bytes, const void* args, cudaStream_t st, int carveout = STEP_CARVEOUT) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -68,10 +73,8 @@ inline int launch(const void* kernel, dim3 grid, int threads, int cluster, int s
   cudaLaunchAttribute attr[3];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  // One split of the SM's memory for all of them: an SM that changes it empties first, so a step that alternates kernels
-  // with and without rings lost the head start (2 requests x 131072 tokens, 256 pages: 41.2 against 36.2 us a step).
   attr[1].id = cudaLaunchAttributePreferredSharedMemoryCarveout;
-  attr[1].val.sharedMemCarveout = 100;
+  attr[1].val.sharedMemCarveout = carveout;
   attr[2].id = cudaLaunchAttributeClusterDimension;
   attr[2].val.clusterDim.x = cluster;
   attr[2].val.clusterDim.y = attr[2].val.clusterDim.z = 1;

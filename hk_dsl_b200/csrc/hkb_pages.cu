@@ -299,8 +299,8 @@ __global__ void __launch_bounds__(WARPS * 32) advance_kernel(const AdvanceArgs a
 // pages of more than 32 tokens the CTA's four warps share it, or a decode step's few large pages would each be one
 // warp's chain of trips to memory: its lanes hold 16-byte chunks of a row, 32 / chunks rows at a time, and fold them
 // with packed minima and maxima that keep a NaN. Bound: bytes (the keys once, two rows a page out). Measured at head size
-// 128, eight kv heads: 4 x 8192 new tokens 14.8 us = 5.1 TB/s; 64 decoding sequences 2.0 us, with pages of 256 tokens
-// 6.9 (15.0 with a warp a page).
+// 128, eight kv heads: 4 x 8192 new tokens 12.4 us = 6.1 TB/s; 64 decoding sequences 2.0 us, with pages of 256 tokens
+// 6.7 (15.0 with a warp a page). Keys through a cp.async ring as the scores': 14.4 to 16.7.
 // ---------------------------------------------------------------------------------
 constexpr int BOUNDS_WARPS = 4;
 
@@ -401,8 +401,14 @@ __global__ void __launch_bounds__(BOUNDS_WARPS * 32) bounds_kernel(const BoundsA
     uint4 v[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {            // a row past the last live one: the last one again
-      const int t = min(t0 + u * RPI + lane / CPR, live - 1);
-      v[u] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)t * a.k_stride_token));
+      const uint8_t* at = src + (int64_t)min(t0 + u * RPI + lane / CPR, live - 1) * a.k_stride_token;
+      // A prompt's keys pass through, with no place in L1 (12.4 against 14.8 us for 4 x 8192 tokens); of a decode step's
+      // few pages the plain load is the quicker (2.0 against 2.4 us for 64 sequences).
+      if (a.q_start)
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(v[u].x), "=r"(v[u].y), "=r"(v[u].z), "=r"(v[u].w) : "l"(at));
+      else
+        v[u] = __ldg(reinterpret_cast<const uint4*>(at));
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
@@ -1004,10 +1010,13 @@ static int page_bounds(void* bounds, int64_t bounds_stride_block, int64_t bounds
   a.table = block_table; a.table_stride = table_stride; a.max_pages = max_pages;
   a.seq_lens = seq_lens; a.q_start = q_start; a.num_seqs = num_seqs; a.num_kv_heads = num_kv_heads; a.page = block_size;
   a.items = (int)items;
+  // Loads in flight live in L1: what reads much keeps the SM's memory for it (4 x 8192 new tokens 12.4 against 15.6 us,
+  // 64 pages of 256 tokens 6.7 against 8.4), a decode step's small launch goes along with the step's other kernels.
+  const int carveout = q_start || share ? 25 : STEP_CARVEOUT;
 #define HKB_BOUNDS(KIND, CPR_) \
   if (kv_dtype == KIND && head_dim * es == CPR_ * 16) { \
     const void* kernel = share ? (const void*)bounds_kernel<KIND, CPR_, true> : (const void*)bounds_kernel<KIND, CPR_, false>; \
-    return launch(kernel, dim3((unsigned)ctas), BOUNDS_WARPS * 32, 1, 0, &a, (cudaStream_t)stream); \
+    return launch(kernel, dim3((unsigned)ctas), BOUNDS_WARPS * 32, 1, 0, &a, (cudaStream_t)stream, carveout); \
   }
   HKB_BOUNDS(HKB_KV_BF16, 8) HKB_BOUNDS(HKB_KV_BF16, 16) HKB_BOUNDS(HKB_KV_BF16, 32)
   HKB_BOUNDS(HKB_KV_F16, 8) HKB_BOUNDS(HKB_KV_F16, 16) HKB_BOUNDS(HKB_KV_F16, 32)
