@@ -193,9 +193,9 @@ __global__ void __launch_bounds__(WARPS * 32) advance_kernel(const AdvanceArgs a
     }
     // This chunk's tokens, dealt to the warps ADV_BLOCKS blocks of 32 at a time (longer runs leave the tokens of many
     // short requests to a few warps). Where they are all one request's, what they share is looked up once; else every
-    // lane looks its request up, block by block. A new page's first position is one of the new tokens', whose lane also writes the page into the table. Once one request gets none,
-    // none of those after it that need pages gets any (the sum runs on), so the pages handed out are the sum's first
-    // ones, in request order.
+    // lane looks its request up, block by block. A new page's first position is one of the new tokens', whose lane also
+    // writes the page into the table. Once one request gets none, none of those after it that need pages gets any (the
+    // sum runs on), so the pages handed out are the sum's first ones, in request order.
     const int rows = clamp31(min((int64_t)total.tokens, a.tokens - before.tokens));     // of the chunk
     const int64_t top = count - 1 - before.need;
     int64_t* const slots = a.slots + before.tokens;
@@ -1052,10 +1052,11 @@ static int page_scores(float* scores, int64_t scores_stride_row, int64_t scores_
   a.table = block_table; a.table_stride = table_stride; a.seq_lens = seq_lens;
   a.page = block_size; a.group = num_q_heads / num_kv_heads; a.scale = scale; a.k_scale = fp8 ? k_scale : nullptr;
   const int64_t tiles = ((int64_t)num_columns + 15) / 16;
-  // as many warps as the machine holds at once, eight an SM, each a CTA of its own
+  // about twice the warps that the machine holds at once (eight an SM, each a CTA of its own): equal shares of a table
+  // are not equal shares of the work where sequences are shorter than it
   int sms = hkb_sm_count(-1);
   if (sms <= 0) sms = 148;
-  const int64_t room = (int64_t)sms * 8, per = (tiles * num_rows * num_kv_heads + room - 1) / room;
+  const int64_t room = (int64_t)sms * 16, per = (tiles * num_rows * num_kv_heads + room - 1) / room;
   a.tiles_per_warp = (int)(per < tiles ? per : tiles);
   const int64_t warps = (tiles + a.tiles_per_warp - 1) / a.tiles_per_warp;
   const dim3 grid((unsigned)((warps + SCORE_WARPS - 1) / SCORE_WARPS), num_kv_heads, num_rows);

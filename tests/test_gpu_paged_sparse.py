@@ -654,6 +654,43 @@ def test_the_torch_ops_are_the_calls():
         assert torch.equal(getattr(a, name), getattr(b, name)), name
 
 
+def test_a_call_behind_another_streams_event_sees_its_writes():
+    """The kernels may take their places while the one before in their stream still runs; what else the stream waits for
+    comes first all the same: another stream's event, a copy, an ordinary kernel."""
+    c = _cache_case([600, 333], d=128, h_kv=2, group=4, seed=61)
+    pages = _random_pages(c, 9)
+    want, _ = _attend(c, pages)
+    k, v, table, lens, pg = c["k"].cuda(), c["v"].cuda(), c["table"].cuda(), _lens(c), pages.cuda()
+    good, host = c["q"].cuda(), c["q"].pin_memory()
+    q, out = torch.zeros_like(good), torch.empty_like(good)
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def call():
+        _ps().paged_sparse_decode(out, q, k, v, table, lens, pg, c["scale"])
+
+    for how in ("event", "copy", "kernel", "event", "kernel"):
+        q.zero_(); out.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(two):
+            call()                                    # the call in front: over the old query
+            if how == "event":
+                with torch.cuda.stream(one):
+                    torch.cuda._sleep(20_000_000)     # some 10 ms
+                    q.copy_(good)
+                    done = one.record_event()
+                two.wait_event(done)
+            elif how == "copy":
+                q.copy_(host, non_blocking=True)
+            else:
+                torch.cuda._sleep(2_000_000)
+                q.add_(good)
+            call()
+            answer = out.clone()                      # an ordinary kernel behind it
+        torch.cuda.synchronize()
+        assert torch.equal(answer, want), how
+
+
 def test_the_same_call_twice_gives_the_same_bits():
     c = _cache_case([4000, 900, 31], d=128, h_kv=2, group=4, seed=21)
     pages = _random_pages(c, 60)
