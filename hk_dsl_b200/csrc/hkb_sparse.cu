@@ -22,8 +22,17 @@ struct SparseArgs {
   float* out_lse;                // (rows, q heads) or null
 };
 
+// CTAs an SM the registers are dealt out for. The rings decide how many fit where a row is 256 bytes or more; with fp8
+// rows of 128 the compiler, told nothing or told one, gave the kernel registers that cost it a CTA or its schedule
+// (128 x 8 items of 128 pages 91.8 and 115 us, told seven 91.0; 2 x 8 of 512, four warps a CTA, 17.8 told nothing, 15.8
+// told one).
+template <class P, int WARPS>
+constexpr int sparse_ctas() {
+  return P::FP8 && WARPS == 2 ? (P::HEAD_DIM == 256 ? 4 : P::HEADS == 8 ? 7 : 5) : 1;
+}
+
 template <class P, int WARPS, bool F16>
-__global__ void __launch_bounds__(WARPS * 32) sparse_kernel(const SparseArgs a) {
+__global__ void __launch_bounds__(WARPS * 32, sparse_ctas<P, WARPS>()) sparse_kernel(const SparseArgs a) {
   extern __shared__ __align__(128) uint8_t hkb_smem[];
   constexpr int D = P::HEAD_DIM, HEADS = P::HEADS, NST = P::STAGES;
   static_assert(NST >= 2, "a stage is computed on while the next is fetched");
