@@ -166,7 +166,7 @@ __device__ __forceinline__ int range_of_warp(const int* ends, int n, int x, int 
 }
 
 template <int WARPS, int EACH>
-__global__ void __launch_bounds__(WARPS * 32) advance_kernel(const AdvanceArgs a) {
+__global__ void __launch_bounds__(WARPS * 32, 1) advance_kernel(const AdvanceArgs a) {
   __shared__ AdvChunk<WARPS, EACH> c;
   after_the_last();
   let_the_next();
@@ -507,7 +507,7 @@ __device__ __forceinline__ float max_nan(float x, float y) {
 }
 
 template <int KIND, int D, int NT>
-__global__ void __launch_bounds__(SCORE_WARPS * 32) scores_kernel(const ScoreArgs a) {
+__global__ void __launch_bounds__(SCORE_WARPS * 32, 8) scores_kernel(const ScoreArgs a) {
   constexpr bool FP8 = KIND == HKB_KV_FP8_E4M3, F16 = KIND != HKB_KV_BF16;   // e4m3 widens to f16 exactly
   using Pr = Pair<F16 ? HKB_KV_F16 : HKB_KV_BF16>;
   constexpr int EPC = FP8 ? 16 : 8;            // elements of a lane's 16-byte chunk
@@ -703,7 +703,7 @@ __device__ __forceinline__ uint32_t score_key(float x) {
 constexpr int SELECT_WARPS = 4;
 
 template <int EACH>
-__global__ void __launch_bounds__(SELECT_WARPS * 32) select_warp_kernel(const SelectArgs a) {
+__global__ void __launch_bounds__(SELECT_WARPS * 32, 1) select_warp_kernel(const SelectArgs a) {
   after_the_last();
   let_the_next();
   const int lane = threadIdx.x & 31;
