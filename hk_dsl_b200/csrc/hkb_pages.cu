@@ -20,7 +20,7 @@ namespace hkb {
 // its share of the tokens and pages; the in-place updates -- the stack's top, the lengths, the count -- come after a
 // cluster barrier, when every CTA has read what it needs of the old state. Deterministic: no atomics.
 // Bound: latency (the scan, then two dependent trips), then the stores of 16 bytes a token. Measured, us a call: 64
-// requests decoding 3.5 (one CTA of 256 threads), 2048 requests with 48 prompts of 2731 tokens 11.7 (a cluster of sixteen
+// requests decoding 3.3 (one CTA of 256 threads), 2048 requests with 48 prompts of 2731 tokens 11.7 (a cluster of sixteen
 // CTAs of 1024 threads; of 512 threads 14.8).
 // ---------------------------------------------------------------------------------
 constexpr int ADV_BLOCKS = 2;                     // 32-token blocks a warp looks up at once
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(BOUNDS_WARPS * 32) bounds_kernel(const BoundsA
 // lane then reads nothing that another one fetched, the copies run through a cp.async ring in which every lane has its
 // own 16-byte places: asynchronous and deep as a walk's ring, without a barrier or a swizzle.
 // Bound: bytes (a summary is 2 rows a page where the attention reads 2 rows a token). Measured: 2 x 8192 pages, eight kv
-// heads of eight query heads, 13.6 us = 4.9 TB/s (loads straight into registers, two tiles a warp: 14.7 to 16; rings in
+// heads of eight query heads, 13.1 us = 5.2 TB/s (loads straight into registers, two tiles a warp: 14.7 to 16; rings in
 // CTAs of four warps instead of one: 17.0, one chain of products a score: 17.3); four sequences of up to 32 pages 1.9 us.
 // ---------------------------------------------------------------------------------
 constexpr int SCORE_WARPS = 1;
