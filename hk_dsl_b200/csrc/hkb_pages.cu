@@ -809,6 +809,7 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectArgs a) {
   constexpr int WORDS = SPAN / 32;
   __shared__ uint32_t above_bits[WORDS], tie_bits[WORDS];
   __shared__ uint64_t before[WORDS];
+  __shared__ int first_of[WORDS];
   __shared__ int s_bin, s_above, s_in;
   constexpr int MINE = SELECT_BINS / THREADS;
   after_the_last();
@@ -842,34 +843,39 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectArgs a) {
 
 #pragma unroll
   for (int i = 0; i < MINE; ++i) hist[tid * MINE + i] = 0;
-  uint32_t least = 0xffffffffu, most = 0u;
+  // columns past the candidates have key 0, which no score has (the least is 2^22)
+  if (RESIDENT)
+#pragma unroll
+    for (int e = 0; e < EACH; ++e)
+      if (e * THREADS + tid >= m) key[e] = 0u;
+  uint32_t least = 0xffffffffu, most = 0u;         // `least` one less than it is, so that key 0 does not count
   for (int p0 = 0; p0 < m; p0 += SPAN) {
     if (!RESIDENT) load(p0, m);
 #pragma unroll
-    for (int e = 0; e < EACH; ++e)
-      if (p0 + e * THREADS + tid < m) { least = min(least, key[e]); most = max(most, key[e]); }
+    for (int e = 0; e < EACH; ++e) { least = min(least, key[e] - 1u); most = max(most, key[e]); }
   }
   least = __reduce_min_sync(0xffffffffu, least);
   most = __reduce_max_sync(0xffffffffu, most);
   if (lane == 0) { ends[0][warp] = least; ends[1][warp] = most; }
   __syncthreads();
-  least = __reduce_min_sync(0xffffffffu, lane < THREADS / 32 ? ends[0][lane] : 0xffffffffu);
+  least = __reduce_min_sync(0xffffffffu, lane < THREADS / 32 ? ends[0][lane] : 0xffffffffu) + 1u;
   most = __reduce_max_sync(0xffffffffu, lane < THREADS / 32 ? ends[1][lane] : 0u);
 
   // Keys from `base` on that are below base + 2^(32 - shift) are undecided; all greater ones are taken.
   uint32_t base = least;
   int shift = __clz(most - least), which = 0;     // 32: they are all one value
-  bool whole = false;                             // all undecided keys are taken
+  bool whole = false, first_pass = true;          // whole: all undecided keys are taken
   while (shift < 32) {
     for (int p0 = 0; p0 < m; p0 += SPAN) {
       if (!RESIDENT) load(p0, m);
 #pragma unroll
       for (int e = 0; e < EACH; ++e) {
-        const uint32_t x = key[e] - base;         // a key below base wraps to a great x
-        if (p0 + e * THREADS + tid < m && key[e] >= base && (x >> (31 - shift)) <= 1u)
+        const uint32_t x = key[e] - base;         // at first every key lies in the range; then one below base wraps to a great x
+        if (first_pass ? key[e] != 0u : key[e] >= base && (x >> (31 - shift)) <= 1u)
           atomicAdd(&hist[(x << shift) >> (32 - SELECT_BITS)], 1);
       }
     }
+    first_pass = false;
     __syncthreads();
     // the bin in which the keys, counted from the top, reach `want`; the bins are cleared for the next pass
     int bins[MINE], mine = 0;
@@ -900,16 +906,40 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectArgs a) {
     shift += SELECT_BITS;                         // 32 and more: the bin is one value
   }
   // Taken: keys above `base`; of those equal to it the first `want` -- or all from it on, where `whole`.
-  uint64_t done = 0;                              // keys above in the upper half, ties in the lower
   const unsigned below = (1u << lane) - 1u;
   static_assert(WORDS <= THREADS, "a word a thread");
+  if (whole) {                                    // nearly always: no ties to count
+    int done = 0;
+    for (int p0 = 0; p0 < m; p0 += SPAN) {
+      if (!RESIDENT) load(p0, m);
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const uint32_t up = __ballot_sync(0xffffffffu, key[e] >= base);
+        if (lane == 0) above_bits[e * (THREADS / 32) + warp] = up;
+      }
+      __syncthreads();
+      const int mine = tid < WORDS ? __popc(above_bits[tid]) : 0;
+      int total;
+      const int incl = done + select_scan<THREADS>(mine, sums[which], total);
+      if (tid < WORDS) first_of[tid] = incl - mine;
+      __syncthreads();
+      which ^= 1;
+      done += total;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int w = e * (THREADS / 32) + warp;
+        if (key[e] >= base) out[first_of[w] + __popc(above_bits[w] & below)] = a.first + p0 + e * THREADS + tid;
+      }
+      if (!RESIDENT) __syncthreads();             // the words are written again
+    }
+    return;
+  }
+  uint64_t done = 0;                              // keys above in the upper half, ties in the lower
   for (int p0 = 0; p0 < m; p0 += SPAN) {
     if (!RESIDENT) load(p0, m);
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-      const bool in_row = p0 + e * THREADS + tid < m;
-      const uint32_t up = __ballot_sync(0xffffffffu, in_row && (whole ? key[e] >= base : key[e] > base));
-      const uint32_t tie = __ballot_sync(0xffffffffu, in_row && !whole && key[e] == base);
+      const uint32_t up = __ballot_sync(0xffffffffu, key[e] > base), tie = __ballot_sync(0xffffffffu, key[e] == base);
       if (lane == 0) { above_bits[e * (THREADS / 32) + warp] = up; tie_bits[e * (THREADS / 32) + warp] = tie; }
     }
     __syncthreads();
@@ -1094,15 +1124,18 @@ static int select_pages(int32_t* pages, int64_t pages_stride_row, int64_t pages_
   if (sms <= 0) sms = 148;
   const dim3 grid(num_rows, num_kv_heads);
   // A warp's steps cost a comparison a key it holds, a CTA's its barriers. Measured, us, (rows x kv heads) of 1000 columns:
-  // 8 of them a warp each 6.5, a CTA each 5.2; 64: 7.2, 5.3; 512: 7.6, 9.7; 4096: 18, 45. Of 500: 4.0, 4.3; 4.5, 4.8.
+  // 8 of them a warp each 6.5, a CTA each 4.2; 64: 7.2, 4.3; 512: 7.5, 9.7 (256 threads); 4096: 18, 45. Of 500: 4.0, 4.3.
   if (num_columns <= 512 || (num_columns <= 1024 && items > 2 * sms)) {
     const void* kernel = num_columns <= 256 ? (const void*)select_warp_kernel<8>
                          : num_columns <= 512 ? (const void*)select_warp_kernel<16> : (const void*)select_warp_kernel<32>;
     return launch(kernel, dim3((unsigned)((items + SELECT_WARPS - 1) / SELECT_WARPS)), SELECT_WARPS * 32, 1, 0, &a, st);
   }
-  // 2000 columns: 8 of them 5.1, 512 10.6 (1024 threads of two keys: 4.9, 16.9). 8000: 8.4 (512 threads of 16: 9.8).
-  if (num_columns <= 2048)
-    return launch(num_columns <= 1024 ? (const void*)select_kernel<256, 4, true> : (const void*)select_kernel<256, 8, true>, grid, 256, 1, 0, &a, st);
+  // A pass costs a thread its keys and the CTA its barriers and its 2048 bins; us, 8 and 512 (rows x kv heads):
+  // 2000 columns 4.7, 9.1 (256 threads of eight keys 6.0, 13.7); 4000: 5.2, 14.1 (of eight keys 6.0, 16.6); 8000: 6.9,
+  // 19.5 (512 threads of sixteen 8.3, 20.2).
+  if (num_columns <= 1024) return launch((const void*)select_kernel<512, 2, true>, grid, 512, 1, 0, &a, st);
+  if (num_columns <= 2048) return launch((const void*)select_kernel<512, 4, true>, grid, 512, 1, 0, &a, st);
+  if (num_columns <= 4096) return launch((const void*)select_kernel<1024, 4, true>, grid, 1024, 1, 0, &a, st);
   const void* kernel = num_columns <= 8192 ? (const void*)select_kernel<1024, 8, true>
                        : num_columns <= 16384 ? (const void*)select_kernel<1024, 16, true> : (const void*)select_kernel<1024, 16, false>;
   return launch(kernel, grid, 1024, 1, 0, &a, st);

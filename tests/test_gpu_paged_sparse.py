@@ -278,7 +278,7 @@ def _select(x, lens, page, budget, first, last):
     return out.cpu()
 
 
-@pytest.mark.parametrize("width", [1, 31, 64, 257, 1000, 2000, 2049, 9000, 16385, 40000])
+@pytest.mark.parametrize("width", [1, 31, 64, 257, 1000, 2000, 2049, 4097, 9000, 16385, 40000])
 @pytest.mark.parametrize("budget, first, last", [(1, 0, 0), (1, 1, 0), (5, 1, 4), (64, 1, 4), (300, 2, 0), (700, 0, 3)])
 def test_select_pages(width, budget, first, last):
     g = torch.Generator().manual_seed(width)
