@@ -20,8 +20,8 @@ namespace hkb {
 // its share of the tokens and pages; the in-place updates -- the stack's top, the lengths, the count -- come after a
 // cluster barrier, when every CTA has read what it needs of the old state. Deterministic: no atomics.
 // Bound: latency (the scan, then two dependent trips), then the stores of 16 bytes a token. Measured, us a call: 64
-// requests decoding 3.3 (one CTA of 256 threads), 2048 requests with 48 prompts of 2731 tokens 11.7 (a cluster of sixteen
-// CTAs of 1024 threads; of 512 threads 14.8).
+// requests decoding 3.3 (one CTA of 256 threads), 2048 requests with 48 prompts of 2731 tokens 11.3 (a cluster of sixteen
+// CTAs of 1024 threads; of 512 threads 12.0).
 // ---------------------------------------------------------------------------------
 constexpr int ADV_BLOCKS = 2;                     // 32-token blocks a warp looks up at once
 
@@ -67,15 +67,21 @@ struct AdvChunk {
   Sums warp[WARPS];
 };
 
-struct AdvRequest { int64_t old, grow, have, want; int status; };
+struct AdvRequest { int old, grow, have, want, status; };
+
+// ceil(tokens / page) for tokens < 2^31, by the multiplication that divides (a division is forty instructions)
+__device__ __forceinline__ int adv_pages(const AdvanceArgs& a, int tokens) {
+  if (tokens == 0) return 0;
+  return a.page == 1 ? tokens : (int)(__umulhi((uint32_t)tokens - 1u, a.page_magic) >> a.page_shift) + 1;
+}
 
 __device__ __forceinline__ AdvRequest adv_request(const AdvanceArgs& a, int r) {
   AdvRequest q = {0, 0, 0, 0, HKB_REQ_OK};
   if (r < a.num_reqs) { q.old = max(a.seq_lens[r], 0); q.grow = a.new_tokens[r]; }
-  const int64_t after = max(q.old + q.grow, (int64_t)0);
-  q.have = min((int64_t)(((uint32_t)q.old + (uint32_t)a.page - 1u) / (uint32_t)a.page), (int64_t)a.max_pages);
-  q.want = (int64_t)(((uint32_t)after + (uint32_t)a.page - 1u) / (uint32_t)a.page);     // old, grow < 2^31
-  if (after > 0x7fffffff) q.want = (int64_t)a.max_pages + 1;
+  q.have = min(adv_pages(a, q.old), a.max_pages);
+  const int after = (int)((uint32_t)q.old + (uint32_t)q.grow);      // old >= 0: only growing can pass 2^31 - 1, and is then negative
+  q.want = adv_pages(a, max(after, 0));
+  if (q.grow > 0 && (after < 0 || q.want > a.max_pages)) q.status = HKB_REQ_TABLE_FULL;
   return q;
 }
 
@@ -118,10 +124,9 @@ __device__ __forceinline__ void adv_chunk(const AdvanceArgs& a, AdvChunk<WARPS, 
   for (int e = 0; e < EACH; ++e) q[e] = adv_request(a, c0 + threadIdx.x * EACH + e);
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
-    if (q[e].grow > 0 && q[e].want > a.max_pages) q[e].status = HKB_REQ_TABLE_FULL;
-    v[e].tokens = clamp31(q[e].grow);
-    v[e].need = q[e].grow > 0 && q[e].status == HKB_REQ_OK ? clamp31(q[e].want - q[e].have) : 0;
-    v[e].give = q[e].grow < 0 ? clamp31(q[e].have - q[e].want) : 0;
+    v[e].tokens = max(q[e].grow, 0);
+    v[e].need = q[e].grow > 0 && q[e].status == HKB_REQ_OK ? max(q[e].want - q[e].have, 0) : 0;
+    v[e].give = q[e].grow < 0 ? max(q[e].have - q[e].want, 0) : 0;
   }
   adv_scan(c, v, incl, total);
   if ((int64_t)before.tokens + total.tokens > a.tokens) {  // some of the rows are missing: those requests take no page either
@@ -138,8 +143,8 @@ __device__ __forceinline__ void adv_chunk(const AdvanceArgs& a, AdvChunk<WARPS, 
     if (v[e].need > 0 && (int64_t)before.need + incl[e].need > count) q[e].status = HKB_REQ_NO_PAGES;
     const int i = threadIdx.x * EACH + e;
     c.ends[i] = incl[e].tokens; c.upto[i] = incl[e].need; c.gives[i] = incl[e].give;
-    c.old[i] = (int)q[e].old;
-    c.have[i] = q[e].status == HKB_REQ_OK ? (int)q[e].have : -1 - (int)q[e].have;
+    c.old[i] = q[e].old;
+    c.have[i] = q[e].status == HKB_REQ_OK ? q[e].have : -1 - q[e].have;
   }
   __syncthreads();
 }
@@ -289,7 +294,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) advance_kernel(const AdvanceArg
       const int r = ch * CHUNK + tid * EACH + e;
       if (r >= a.num_reqs) continue;
       if (!once) { q[e] = adv_request(a, r); q[e].status = a.status[r]; }      // which this thread wrote
-      a.seq_lens[r] = (int)(q[e].status == HKB_REQ_OK ? max(q[e].old + q[e].grow, (int64_t)0) : q[e].old);
+      a.seq_lens[r] = q[e].status == HKB_REQ_OK ? max(q[e].old + q[e].grow, 0) : q[e].old;
     }
 }
 
@@ -317,6 +322,7 @@ struct BoundsArgs {
   const int* q_start;              // null: one new token a sequence
   int num_seqs, num_kv_heads, page;
   int items;                       // (sequence, page) pairs the grid covers
+  bool many;                       // more than the machine holds at once
 };
 
 template <int KIND>
@@ -402,9 +408,9 @@ __global__ void __launch_bounds__(BOUNDS_WARPS * 32) bounds_kernel(const BoundsA
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {            // a row past the last live one: the last one again
       const uint8_t* at = src + (int64_t)min(t0 + u * RPI + lane / CPR, live - 1) * a.k_stride_token;
-      // A prompt's keys pass through, with no place in L1 (12.4 against 14.8 us for 4 x 8192 tokens); of a decode step's
-      // few pages the plain load is the quicker (2.0 against 2.4 us for 64 sequences).
-      if (a.q_start)
+      // Many pages' keys pass through, with no place in L1 (12.4 against 14.8 us for 4 x 8192 tokens); of a decode step's
+      // few the plain load is the quicker (2.0 against 2.4 us for 64 sequences).
+      if (a.many)
         asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                      : "=r"(v[u].x), "=r"(v[u].y), "=r"(v[u].z), "=r"(v[u].w) : "l"(at));
       else
@@ -1042,7 +1048,10 @@ static int page_bounds(void* bounds, int64_t bounds_stride_block, int64_t bounds
   a.items = (int)items;
   // Loads in flight live in L1: what reads much keeps the SM's memory for it (4 x 8192 new tokens 12.4 against 15.6 us,
   // 64 pages of 256 tokens 6.7 against 8.4), a decode step's small launch goes along with the step's other kernels.
-  const int carveout = q_start || share ? 25 : STEP_CARVEOUT;
+  int sms = hkb_sm_count(-1);
+  if (sms <= 0) sms = 148;
+  a.many = items * num_kv_heads * (((int64_t)block_size + 15) / 16) > 64 * sms;        // of 16 tokens
+  const int carveout = a.many || share ? 25 : STEP_CARVEOUT;
 #define HKB_BOUNDS(KIND, CPR_) \
   if (kv_dtype == KIND && head_dim * es == CPR_ * 16) { \
     const void* kernel = share ? (const void*)bounds_kernel<KIND, CPR_, true> : (const void*)bounds_kernel<KIND, CPR_, false>; \

@@ -59,7 +59,7 @@ def advance_ref(table, lens, new, free, count, page, rows):
         elif n < 0:
             want = ceil_div(after, page)
             back += table[i][want:have]
-        for j in range(max(0, n)):
+        for j in range(min(max(0, n), max(0, rows - t0))):
             if t0 + j < rows:
                 pos = old + j
                 block = table[i][pos // page] if st == OK else -1

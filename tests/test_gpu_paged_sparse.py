@@ -91,6 +91,20 @@ def test_advance_tables_many_steps_keep_every_page():
         assert sorted(owned + free[:count]) == list(range(pool))
 
 
+def test_advance_tables_at_the_ends_of_its_integers():
+    """Lengths and demands near 2^31, and a demand that goes past it."""
+    top = 2 ** 31 - 1
+    for page, width in ((1, 3), (16, 3), (2 ** 30, 2), (top, 1)):
+        lens = [top, 5, 0, -3, 7, 2, top]
+        new = [top, top, -top - 1, 1, top - 7, 0, -top]
+        table = [[40 + i] * width for i in range(7)]
+        want = orc.advance_ref(table, lens, new, [9, 8, 7, 6], 4, page, 4)
+        got = _advance(table, lens, new, [9, 8, 7, 6], 4, page, 4)
+        starts = [min(x, top) for x in want[6]]       # held at 2^31 - 1
+        for name, g, w in zip(("table", "lens", "free", "count", "slots", "positions", "starts", "status"), got, want[:6] + (starts, want[7])):
+            assert g == w, (page, name)
+
+
 def test_advance_tables_without_requests_and_past_the_stacks_capacity():
     ps = _ps()
     e = lambda *s, d=torch.int32: torch.full(s, 9, dtype=d, device="cuda")  # noqa: E731
