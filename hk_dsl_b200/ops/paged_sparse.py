@@ -16,7 +16,9 @@ the GPU from the requests' lengths. A step of a layer:
 Caches, queries and tables are those of `hk_dsl_b200.ops.paged`: `(blocks, block_size, kv_heads, head_dim)` views of any
 strides in bf16, fp16 or fp8-e4m3, `(rows, q_heads, head_dim)` queries, int32 tables and lengths, row i of the query
 belonging to row i of the table. Every call is one launch on torch's current stream; it allocates nothing, reads
-nothing back and can be captured into a CUDA graph. There is no fallback: a call the kernels do not take raises.
+nothing back and can be captured into a CUDA graph. A tensor that a call writes overlaps neither itself (`expand`) nor
+another one of the call's; a page is read by as many rows as list it. There is no fallback: a call the kernels do not
+take raises.
 """
 
 from __future__ import annotations
@@ -67,17 +69,17 @@ def _page_size(block_size: int) -> int:
     return int(block_size)
 
 
-def _tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, rows: int) -> int:
-    """The checked table's width."""
-    if block_tables.dtype is not _I32 or seq_lens.dtype is not _I32 or block_tables.dim() != 2 or seq_lens.dim() != 1 \
-            or not block_tables.is_contiguous() or not seq_lens.is_contiguous():
-        _index("block_tables", block_tables, 2)       # which of them, and whether a strided one is one the kernels take
+def _tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, rows: int):
+    """The checked table's width and the stride of its rows."""
+    shape, strides, lens = block_tables.shape, block_tables.stride(), seq_lens.shape
+    if block_tables.dtype is not _I32 or seq_lens.dtype is not _I32 or len(shape) != 2 or strides[1] != 1 \
+            or seq_lens.stride() != (1,):
+        _index("block_tables", block_tables, 2)       # which of them, and whether it is one the kernels take all the same
         _index("seq_lens", seq_lens, 1)
-    have, width = block_tables.shape
-    if have < rows or seq_lens.shape[0] < rows:
-        raise ValueError(f"{_WHO}: block_tables {tuple(block_tables.shape)} and seq_lens {tuple(seq_lens.shape)} "
-                         f"for {rows} rows")
-    return width
+    have, width = shape
+    if have < rows or lens[0] < rows:
+        raise ValueError(f"{_WHO}: block_tables {tuple(shape)} and seq_lens {tuple(lens)} for {rows} rows")
+    return width, strides[0]
 
 
 def page_bounds(key_cache: torch.Tensor) -> torch.Tensor:
@@ -103,15 +105,16 @@ def advance_tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, new_token
     or `REQ_NO_ROWS` keeps its length, gets no page, and its rows get slot -1. A page belongs to one request."""
     _index("block_tables", block_tables, 2)
     for t in (seq_lens, new_tokens, free_pages, free_count, query_start_loc, status):
-        if t.dtype is not _I32 or t.dim() != 1 or not t.is_contiguous():
+        if t.dtype is not _I32 or t.stride() != (1,):
             for name, x in (("seq_lens", seq_lens), ("new_tokens", new_tokens), ("free_pages", free_pages),
                             ("free_count", free_count), ("query_start_loc", query_start_loc), ("status", status)):
                 _index(name, x, 1)
-    _index("slot_mapping", slot_mapping, 1, _I64)
-    _index("positions", positions, 1, _I64)
+    if slot_mapping.dtype is not _I64 or positions.dtype is not _I64 or slot_mapping.stride() != (1,) or positions.stride() != (1,):
+        _index("slot_mapping", slot_mapping, 1, _I64)
+        _index("positions", positions, 1, _I64)
     n, = seq_lens.shape
     have, width = block_tables.shape
-    stride = block_tables.stride(0)
+    stride = block_tables.stride()[0]
     rows, = slot_mapping.shape
     if have < n or new_tokens.shape[0] < n or status.shape[0] < n or query_start_loc.shape[0] < n + 1:
         raise ValueError(f"{_WHO}: {n} requests (seq_lens) with block_tables {tuple(block_tables.shape)}, new_tokens "
@@ -182,7 +185,7 @@ def update_page_bounds(bounds: torch.Tensor, key_cache: torch.Tensor, block_tabl
         raise ValueError(f"{_WHO}: bounds {tuple(bounds.shape)} {bounds.dtype} beside a key cache {tuple(key_cache.shape)} "
                          f"{key_cache.dtype}")
     n = seq_lens.shape[0]
-    width = _tables(block_tables, seq_lens, n)
+    width, stride = _tables(block_tables, seq_lens, n)
     starts = 0
     if query_start_loc is not None:
         _index("query_start_loc", query_start_loc, 1)
@@ -194,7 +197,7 @@ def update_page_bounds(bounds: torch.Tensor, key_cache: torch.Tensor, block_tabl
     stream = _on(bounds, key_cache, block_tables, seq_lens, query_start_loc)
     rc = _lib.load().hkb_page_bounds(_lib.PAGE_BOUNDS(
         bounds.data_ptr(), bs[0], bs[1], bshape[0], key_cache.data_ptr(), ks[0], ks[1], ks[2], nb,
-        block_tables.data_ptr(), block_tables.stride(0), width, seq_lens.data_ptr(), starts, n, num_tokens or 0, hkv, d,
+        block_tables.data_ptr(), stride, width, seq_lens.data_ptr(), starts, n, num_tokens or 0, hkv, d,
         page, code), stream)
     if rc:
         _lib.check("hkb_page_bounds", rc)
@@ -234,7 +237,7 @@ def page_scores(scores: torch.Tensor, query: torch.Tensor, bounds: torch.Tensor,
     `query` (rows, q_heads, head_dim); `bounds` from `update_page_bounds`."""
     (rows, hq, d), qs = _query(query)
     (nb, hkv, _, bd), bs = _bounds_strides(bounds)
-    width = _tables(block_tables, seq_lens, rows)
+    width, stride = _tables(block_tables, seq_lens, rows)
     ss = scores.stride()
     if bd != d or hkv < 1 or hq % hkv:
         raise ValueError(f"{_WHO}: query {tuple(query.shape)} beside bounds {tuple(bounds.shape)}")
@@ -246,7 +249,7 @@ def page_scores(scores: torch.Tensor, query: torch.Tensor, bounds: torch.Tensor,
     stream = _on(query, scores, bounds, block_tables, seq_lens, k_scale)
     rc = _lib.load().hkb_page_scores(_lib.PAGE_SCORES(
         scores.data_ptr(), ss[0], ss[1], width, query.data_ptr(), qs[0], qs[1], bounds.data_ptr(), bs[0], bs[1], nb,
-        block_tables.data_ptr(), block_tables.stride(0), seq_lens.data_ptr(), rows, hq, hkv, d, page, code,
+        block_tables.data_ptr(), stride, seq_lens.data_ptr(), rows, hq, hkv, d, page, code,
         _scale_ptr(k_scale, code == _lib.KV_FP8_E4M3, "k_scale") or 0, scale), stream)
     if rc:
         _lib.check("hkb_page_scores", rc)
@@ -259,15 +262,17 @@ def select_pages(pages: torch.Tensor, scores: torch.Tensor, seq_lens: torch.Tens
     `first` and the `last` pages of the row's sequence and then those of the greatest `scores` (rows, kv_heads, columns)
     fp32, ties to the lowest page, NaN above all numbers. A row with no more pages than the budget gets them all.
     The entries number the row's pages (columns of its block table), as `paged_sparse_decode` reads them."""
-    _index("pages", pages, 3)
-    _index("seq_lens", seq_lens, 1)
-    rows, hkv, budget = pages.shape
-    shape, ss, ps = scores.shape, scores.stride(), pages.stride()
+    pshape, ps, lens = pages.shape, pages.stride(), seq_lens.shape
+    if pages.dtype is not _I32 or seq_lens.dtype is not _I32 or len(pshape) != 3 or ps[2] != 1 or seq_lens.stride() != (1,):
+        _index("pages", pages, 3)
+        _index("seq_lens", seq_lens, 1)
+    rows, hkv, budget = pshape
+    shape, ss = scores.shape, scores.stride()
     if scores.dtype is not _F32 or len(shape) != 3 or shape[0] != rows or shape[1] != hkv or (shape[2] > 1 and ss[2] != 1):
         raise ValueError(f"{_WHO}: scores is {tuple(shape)} {scores.dtype} beside pages {tuple(pages.shape)}; "
                          f"({rows}, {hkv}, columns) float32 with contiguous columns needed")
-    if seq_lens.shape[0] < rows:
-        raise ValueError(f"{_WHO}: {seq_lens.shape[0]} lengths for {rows} rows")
+    if lens[0] < rows:
+        raise ValueError(f"{_WHO}: {lens[0]} lengths for {rows} rows")
     if first < 0 or last < 0 or first + last > budget:
         raise ValueError(f"{_WHO}: first {first} and last {last} pages of a budget of {budget}")
     page = _page_size(block_size)
@@ -297,10 +302,11 @@ def paged_sparse_decode(out: torch.Tensor, query: torch.Tensor, key_cache: torch
                          f"{tuple(qshape)} {query.dtype}")
     rows, hq, d = qshape
     (nb, page, hkv, cd), ks, vs = _cache_strides(key_cache, value_cache)
-    width = _tables(block_tables, seq_lens, rows)
-    _index("pages", pages, 3)
-    listed, heads, budget = pages.shape
-    ps = pages.stride()
+    width, stride = _tables(block_tables, seq_lens, rows)
+    pshape, ps = pages.shape, pages.stride()
+    if pages.dtype is not _I32 or len(pshape) != 3 or ps[2] != 1:
+        _index("pages", pages, 3)
+    listed, heads, budget = pshape
     if cd != d or listed != rows or heads != hkv:
         raise ValueError(f"{_WHO}: pages is {tuple(pages.shape)} beside query {tuple(qshape)} and key_cache "
                          f"{tuple(key_cache.shape)}; ({rows}, {hkv}, budget) and one head size needed")
@@ -316,7 +322,7 @@ def paged_sparse_decode(out: torch.Tensor, query: torch.Tensor, key_cache: torch
     rc = _lib.load().hkb_paged_sparse_decode(_lib.SPARSE_DECODE(
         out.data_ptr(), os[0], os[1], lse, query.data_ptr(), qs[0], qs[1],
         key_cache.data_ptr(), ks[0], ks[1], ks[2], nb, value_cache.data_ptr(), vs[0], vs[1], vs[2], nb,
-        block_tables.data_ptr(), block_tables.stride(0), width, seq_lens.data_ptr(), pages.data_ptr(), ps[0], ps[1], budget,
+        block_tables.data_ptr(), stride, width, seq_lens.data_ptr(), pages.data_ptr(), ps[0], ps[1], budget,
         rows, hq, hkv, d, page, code, _scale_ptr(k_scale, fp8, "k_scale") or 0, _scale_ptr(v_scale, fp8, "v_scale") or 0,
         scale), stream)
     if rc:
