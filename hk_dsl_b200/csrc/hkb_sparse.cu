@@ -199,18 +199,32 @@ __global__ void __launch_bounds__(WARPS * 32, sparse_ctas<P, WARPS>()) sparse_ke
 //   bf16, 64 x 8 items of 64 pages: 1 CTA 45.5, 2 48.4, 4 55.8 (two warps); 1 CTA of four 46.9, of eight 53.0
 //   bf16, 16 x 8 items of 256 pages: 1 CTA 67.0, 2 47.6, 4 45.7, 8 49.5; 2 x 8 of 1024: 8 CTAs 37.0, of four warps 28.4
 //   fp8, 48 x 8 items of 64 pages (rings half the size, so twice the CTAs fit): 1 CTA 29.1, 2 22.6, 4 28.9
-// Short lists do not pay for the wider clusters: fp8, 16 x 8 items of 16 pages: 4 CTAs 7.1, 8 8.5.
+// Short lists do not pay for the wider clusters: fp8, 16 x 8 items of 16 pages: 4 CTAs 7.1, 8 8.5; bf16, 8 x 8 of 32: 4
+// CTAs 6.4, 8 7.1; with eight heads they pay for a pair from 2048 channels on: fp8, 64 x 8 items of 8 pages 1 CTA 6.8, 2
+// 8.1; of 16 11.9, 11.2; of 48 25.8, 22.0 (sixteen heads, of 16: 18.7, 23.2: registers). Nor for a cluster at all: its
+// barriers and peers' memory cost 1.2 us, half that with an SM a CTA, and a tile costs a warp 0.33, 0.43, 0.66 us (head
+// size 64, 128, 256, eight heads; twice that sixteen). So one CTA of four warps, where the items are one wave of those
+// (registers let three in, two with sixteen heads) and the tiles a warp has more of, tiles (1/4 - 1/2c), cost less:
+//   bf16, cluster / four warps: 1 x 8 items of 4 pages 4.3 / 3.6, of 8 4.5 / 4.0, of 32 5.2 / 6.6; 16 x 8 of 8 5.8 / 4.3, of
+//   24 7.2 / 7.1, 32 x 8 of 16 8.9 / 8.2; head size 256, 1 x 8 of 8 5.3 / 5.4, 16 x 8 of 8 7.2 / 6.2
+// and instead of a CTA of two warps where each of the four has four tiles (fp8, 48 x 8 items of 16 pages 10.4 / 7.6, of 32
+// 17.1 / 13.2; head size 64, of 8 4.9 / 5.4).
 struct SparseShape { int ctas, warps; };
-static SparseShape sparse_shape(int rows, int kv_heads, int64_t tiles, int ring_bytes) {
+static SparseShape sparse_shape(int rows, int kv_heads, int64_t tiles, int ring_bytes, int head_dim, int heads) {
   int sms = hkb_sm_count(-1);
   if (sms <= 0) sms = 148;
   SparseShape s = {1, 2};
   const int64_t items = (int64_t)rows * kv_heads;
   int fit = (227 << 10) / (2 * ring_bytes + 1024);
   fit = fit > 8 ? 8 : fit;
-  if (tiles < 64 && fit > 4) fit = 4;
-  while (s.ctas < 8 && items * s.ctas * 2 <= (int64_t)fit * sms && tiles > s.ctas * 2) s.ctas *= 2;
-  if (s.ctas == 8 && items * 8 <= 2 * sms && tiles > 128) s.warps = 4;
+  const int wide = tiles < 64 && fit > 4 ? 4 : fit, pair = heads > 8 || tiles * head_dim < 2048 ? wide : fit;
+  while (s.ctas < 8 && items * s.ctas * 2 <= (int64_t)(s.ctas == 1 ? pair : wide) * sms && tiles > s.ctas * 2) s.ctas *= 2;
+  if (s.ctas == 8 && items * 8 > 2 * sms && tiles < 64) s.ctas = 4;
+  const int rings = (227 << 10) / (4 * ring_bytes + 1024), regs = heads == 8 ? 3 : 2;
+  const bool wave = items <= (int64_t)(rings < regs ? rings : regs) * sms;
+  const int cost = (64 + head_dim / 2) * (heads / 8), bear = (items * s.ctas > sms ? 1408 : 704) * s.ctas;
+  if (wave && (s.ctas == 1 ? tiles >= 16 : tiles * (s.ctas - 2) * cost <= bear)) s = {1, 4};
+  else if (s.ctas == 8 && items * 8 <= 2 * sms && tiles > 128) s.warps = 4;
   return s;
 }
 
@@ -235,7 +249,8 @@ static int dispatch_sparse(const SparseArgs& a, int rows, cudaStream_t st) {
   // Three stages a ring whatever a tile's size: head size 256, bf16, 64 x 8 items of 32 pages 48.8 us on two CTAs an SM
   // against 55.7 on three of two stages; four stages of fp8 33.6 against 27.6 (16 x 8 items of 16 pages of 256 tokens).
   constexpr int NST = 3;
-  const SparseShape shape = sparse_shape(rows, a.d.num_kv_heads, (int64_t)a.budget * a.d.tiles_per_page, SparseWorker<D, KIND, NT, NST>::RING_SMEM);
+  using P = SparseWorker<D, KIND, NT, NST>;
+  const SparseShape shape = sparse_shape(rows, a.d.num_kv_heads, (int64_t)a.budget * a.d.tiles_per_page, P::RING_SMEM, D, P::HEADS);
   return shape.warps == 2 ? launch_sparse<D, KIND, NT, NST, 2>(a, rows, shape.ctas, st) : launch_sparse<D, KIND, NT, NST, 4>(a, rows, shape.ctas, st);
 }
 template <int KIND, int NT>
