@@ -320,6 +320,7 @@ struct BoundsArgs {
   int max_pages;
   const int* seq_lens;
   const int* q_start;              // null: one new token a sequence
+  int tokens;                      // the step's rows; a start past them counts as it
   int num_seqs, num_kv_heads, page;
   int items;                       // (sequence, page) pairs the grid covers
   bool many;                       // more than the machine holds at once
@@ -368,20 +369,22 @@ __global__ void __launch_bounds__(BOUNDS_WARPS * 32) bounds_kernel(const BoundsA
   if (item >= a.items) return;
 
   // which page of which sequence. With query starts, sequence r has the items from start[r] / page + 2 r on:
-  // its q new tokens touch at most q / page + 2 pages, and so many items it has.
+  // its q new tokens touch at most q / page + 2 pages, and so many items it has. Requests that got no rows leave starts
+  // past the step's; held at the rows, everyone's items lie in the grid, two at least.
   int r = item, page;
   int len;
   if (a.q_start) {
+    auto start = [&](int i) { return min(max(__ldg(a.q_start + i), 0), a.tokens); };
     int lo = 0, hi = a.num_seqs;                  // the last r whose items begin at or before this one is in [lo, hi)
     while (hi - lo > 1) {                         // 32 candidates at once
       const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-      const bool below = at < hi && __ldg(a.q_start + at) / a.page + 2 * at <= item;
+      const bool below = at < hi && start(at) / a.page + 2 * at <= item;
       const int m = max(__popc(__ballot_sync(0xffffffffu, below)), 1);
       lo += (m - 1) * step;
       hi = min(hi, lo + step);
     }
     r = lo;
-    const int s0 = __ldg(a.q_start + r), q = __ldg(a.q_start + r + 1) - s0;
+    const int s0 = start(r), q = start(r + 1) - s0;
     len = __ldg(a.seq_lens + r);
     if (len <= 0) return;
     const int64_t k = (int64_t)item - (s0 / a.page + 2 * (int64_t)r);
@@ -1044,7 +1047,8 @@ static int page_bounds(void* bounds, int64_t bounds_stride_block, int64_t bounds
   const int64_t nb = kc.num_blocks < bounds_blocks ? kc.num_blocks : bounds_blocks;
   a.num_blocks = nb > 0x7fffffff ? 0x7fffffff : (int)nb;
   a.table = block_table; a.table_stride = table_stride; a.max_pages = max_pages;
-  a.seq_lens = seq_lens; a.q_start = q_start; a.num_seqs = num_seqs; a.num_kv_heads = num_kv_heads; a.page = block_size;
+  a.seq_lens = seq_lens; a.q_start = q_start; a.tokens = num_tokens > 0x7fffffff ? 0x7fffffff : (int)num_tokens;
+  a.num_seqs = num_seqs; a.num_kv_heads = num_kv_heads; a.page = block_size;
   a.items = (int)items;
   // Loads in flight live in L1: what reads much keeps the SM's memory for it (4 x 8192 new tokens 12.4 against 15.6 us,
   // 64 pages of 256 tokens 6.7 against 8.4), a decode step's small launch goes along with the step's other kernels.

@@ -174,9 +174,10 @@ def update_page_bounds(bounds: torch.Tensor, key_cache: torch.Tensor, block_tabl
     and the greatest key of every channel over the page's tokens below the sequence's length.
 
     To be called behind the cache write. Without `query_start_loc` every sequence has one new token; with it (int32,
-    sequences + 1, from `advance_tables`) sequence i has `query_start_loc[i + 1] - query_start_loc[i]`, and `num_tokens`, a
-    host number, is at least its last entry (the step's rows). A sequence without new tokens has its last page summarised
-    again: it holds fewer tokens if the sequence was shortened. `bounds` is of the cache's type: nothing is rounded. Pages
+    sequences + 1, from `advance_tables`) sequence i has `query_start_loc[i + 1] - query_start_loc[i]`, of those that lie
+    below `num_tokens`, the step's rows (a host number): the starts run on past it where `advance_tables` refused a
+    request for rows. A sequence without new tokens has its last page summarised again: it holds fewer tokens if the
+    sequence was shortened. `bounds` is of the cache's type: nothing is rounded. Pages
     are read from the cache as it is, so a call may be repeated; sequences of length 0 are left out."""
     (nb, page, hkv, d), ks, _ = _cache_strides(key_cache)
     bshape, bs = _bounds_strides(bounds)

@@ -502,11 +502,12 @@ int hkb_advance_tables(const hkb_advance_t* args, void* stream);
  * Page summaries for a decode over selected pages: bounds[b, h, 0, :] and bounds[b, h, 1, :] become the least and
  * the greatest key of every channel of kv head h over the tokens of page b below its sequence's length. Of
  * sequence i the pages that hold its last max(1, q_start[i+1] - q_start[i]) tokens are summarised (q_start NULL: its
- * last token), from the cache as it is: call it behind the cache write of those tokens. A sequence without new tokens
- * has its last page summarised again, which holds fewer tokens if the sequence was shortened. bounds has the cache's element type (values are kept exactly, fp8 ones as stored); its last two axes
- * are contiguous, head_dim each. A NaN key makes the channel's bounds NaN. Page ids outside
- * [0, min(bounds_blocks, k_cache.num_blocks)) are skipped. num_tokens: an upper bound of q_start[num_seqs], which
- * must not be below it. block_size is any positive number.
+ * last token), from the cache as it is: call it behind the cache write of those tokens. num_tokens: the step's rows;
+ * tokens at or past row num_tokens are none (hkb_advance_tables counts those of requests that got no rows), so an entry
+ * of q_start past it counts as it. A sequence without new tokens has its last page summarised again, which holds fewer
+ * tokens if the sequence was shortened. bounds has the cache's element type (values are kept exactly, fp8 ones as
+ * stored); its last two axes are contiguous, head_dim each. A NaN key makes the channel's bounds NaN. Page ids outside
+ * [0, min(bounds_blocks, k_cache.num_blocks)) are skipped. block_size is any positive number.
  */
 typedef struct {
   void* bounds;
