@@ -2,7 +2,7 @@
 // a page's summary, the summaries' scores against a query, the budget's best pages.
 #include "hkb_common.cuh"
 #include "hkb_cluster.cuh"
-#include "hkb_walk_mma.cuh"
+#include "hkb_sparse.cuh"
 
 extern thread_local int hkb_tls_cuda_error;
 
@@ -581,8 +581,6 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32, 8) scores_kernel(const Score
       }
     unit[nt] = 1.f;
     if (FP8) {
-      // bf16 -> f16: the head's values are brought below 2^14 by a power of two (exact), so that none overflows
-      // and what falls under f16's range is 2^-38 of the largest
       float top = 0.f;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s)
@@ -591,14 +589,13 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32, 8) scores_kernel(const Score
           top = fmaxf(top, fmaxf(fabsf(bf16lo(qf[nt][s][i])), fabsf(bf16hi(qf[nt][s][i]))));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = min(max((int)(__float_as_uint(top) >> 23), 14), 253);   // biased exponent; inf and zero keep a finite factor
-      const float down = __uint_as_float((uint32_t)(267 - e) << 23);         // 2^(13 - (e - 127)), at most 2^126
-      unit[nt] = __uint_as_float((uint32_t)(e - 13) << 23);
+      const F16Scale f = f16_scale(top);
+      unit[nt] = f.up;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s)
 #pragma unroll
         for (int i = 0; i < EPC / 2; ++i)
-          qf[nt][s][i] = pack_f16x2(bf16lo(qf[nt][s][i]) * down, bf16hi(qf[nt][s][i]) * down);
+          qf[nt][s][i] = pack_f16x2(bf16lo(qf[nt][s][i]) * f.down, bf16hi(qf[nt][s][i]) * f.down);
     }
   }
   const float factor = a.scale * (a.k_scale ? __ldg(a.k_scale) : 1.f);

@@ -99,13 +99,13 @@ __global__ void __launch_bounds__(WARPS * 32, sparse_ctas<P, WARPS>()) sparse_ke
   for (int k = 0; k < NST - 1; ++k) queue[k] = issue(k);
 
   typename P::State st;
-  P::Walk::begin(st, a.d, row, hq0, nh, lane, qs);
+  P::begin(st, a.d, row, hq0, nh, lane, qs);
   int sc = 0, sl = NST - 1;
   while (queue[0] >= 0) {
     cp_async_wait<NST - 2>();
     __syncwarp();
     const int t = issue(sl);     // over the tile before
-    P::step(st, ring + sc * P::STAGE_BYTES, queue[0], seq_len, queue[0] + TILE_TOKENS > seq_len, lane, qs);
+    P::step(st, ring + sc * P::STAGE_BYTES, queue[0], seq_len, queue[0] + TILE_TOKENS > seq_len, lane);
 #pragma unroll
     for (int k = 0; k + 1 < NST - 1; ++k) queue[k] = queue[k + 1];
     queue[NST - 2] = t;

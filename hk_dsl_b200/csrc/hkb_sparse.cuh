@@ -14,20 +14,71 @@
 
 namespace hkb {
 
+// A head of a bf16 query as f16, for an fp8 cache's products: its values times the power of two that brings the greatest
+// magnitude `top` into [2^13, 2^14). That is exact, none overflows whatever the query's range, and what falls under f16's
+// is off by 2^-38 of the greatest at most. `up` undoes it. (top zero, subnormal or infinite: a finite pair all the same.)
+struct F16Scale { float down, up; };
+__device__ __forceinline__ F16Scale f16_scale(float top) {
+  const int e = min(max((int)(__float_as_uint(top) >> 23), 14), 253);   // biased exponent
+  return {__uint_as_float((uint32_t)(267 - e) << 23), __uint_as_float((uint32_t)(e - 13) << 23)};
+}
+
 template <int D, int KIND, int NT, int NST>
 struct SparseWorker {
   static constexpr bool FP8 = KIND == HKB_KV_FP8_E4M3, F16 = KIND != HKB_KV_BF16;   // e4m3 is widened to f16
-  // queries, accumulators and the partial's layout are the walk's
+  // accumulators and the partial's layout are the walk's
   using Walk = typename std::conditional<FP8, WalkMMAF8<D, NT, NST, 1>, WalkMMA<D, false, NT, 1, NST, KIND == HKB_KV_F16>>::type;
-  using State = typename Walk::State;
+  struct State : Walk::State { float qs[NT][2]; };     // and what a column's products are multiplied by: logits in units of ln 2
   using Loader = typename Walk::Loader;
   static constexpr int HEAD_DIM = D, HEADS = NT * 8, STAGES = NST, KD = D / 16;
   static constexpr int STAGE_BYTES = 2 * Loader::TILE_BYTES;    // K, then V
   static constexpr int RING_SMEM = NST * STAGE_BYTES;
   static constexpr float RESCALE_LOG2 = 8.f;
 
+  // As the walk's, but for an fp8 cache's query, which the walk cuts at f16's range: here each head is scaled into it, and
+  // NaN and infinities stay what they are.
+  __device__ static __forceinline__ void begin(State& st, const DecodeArgs& a, int row, int hq0, int nh, int lane, float qs) {
+    Walk::begin(st, a, row, hq0, nh, lane, qs);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      st.qs[nt][0] = st.qs[nt][1] = qs;
+      if constexpr (FP8) {
+        const int h = nt * 8 + (lane >> 2), t = lane & 3;
+        const uint4* qp = reinterpret_cast<const uint4*>(a.q + (int64_t)row * a.q_stride_tok + (int64_t)(hq0 + h) * a.q_stride_head);
+        uint32_t w[KD][2];                           // dims 32 s + 8 t .. + 7: chunks 2 s and 2 s + 1
+        float top = 0.f;
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) {
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (h < nh) v = __ldg(qp + s * 4 + t);
+          w[2 * s][0] = v.x; w[2 * s][1] = v.y; w[2 * s + 1][0] = v.z; w[2 * s + 1][1] = v.w;
+        }
+#pragma unroll
+        for (int kc = 0; kc < KD; ++kc)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) top = fmaxf(top, fmaxf(fabsf(bf16lo(w[kc][i])), fabsf(bf16hi(w[kc][i]))));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const F16Scale f = f16_scale(top);
+#pragma unroll
+        for (int kc = 0; kc < KD; ++kc)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) st.qb[nt][kc][i] = pack_f16x2(bf16lo(w[kc][i]) * f.down, bf16hi(w[kc][i]) * f.down);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x = qs * __shfl_sync(0xffffffffu, f.up, (2 * t + c) * 4);
+          // neither 0, which makes NaN of a masked -inf, nor infinite, which makes NaN of a product of 0: products are
+          // below 2^31, so under 2^-126 the logits are nothing
+          if (fabsf(x) < 0x1p-126f) x = 0x1p-126f;
+          if (x > 0x1.fffffep127f && qs <= 0x1.fffffep127f) x = 0x1.fffffep127f;
+          st.qs[nt][c] = x;
+        }
+      }
+    }
+  }
+
   // One tile, from its first token `tok`; `tail`: it ends behind the sequence.
-  __device__ static __forceinline__ void step(State& st, uint32_t ktile, int tok, int seq_len, bool tail, int lane, float qs) {
+  __device__ static __forceinline__ void step(State& st, uint32_t ktile, int tok, int seq_len, bool tail, int lane) {
     const uint32_t vtile = ktile + Loader::TILE_BYTES;
     if (tail) {     // V rows past the sequence: their weight is 0, but 0 * NaN is NaN
       Walk::scrub_tail(vtile, tok, seq_len, lane);
@@ -74,7 +125,7 @@ struct SparseWorker {
       top[nt][1] = fmaxf(sc[nt][1], sc[nt][3]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        top[nt][c] *= qs;                          // qs > 0
+        top[nt][c] *= st.qs[nt][c];                // > 0
         over |= top[nt][c] > st.m[nt][c] + RESCALE_LOG2;
       }
     }
@@ -97,8 +148,9 @@ struct SparseWorker {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float mu0 = st.m[nt][0] == -INFINITY ? 0.f : -st.m[nt][0], mu1 = st.m[nt][1] == -INFINITY ? 0.f : -st.m[nt][1];
-      const float p0 = fast_exp2(fmaf(sc[nt][0], qs, mu0)), p1 = fast_exp2(fmaf(sc[nt][1], qs, mu1));
-      const float p2 = fast_exp2(fmaf(sc[nt][2], qs, mu0)), p3 = fast_exp2(fmaf(sc[nt][3], qs, mu1));
+      const float qs0 = st.qs[nt][0], qs1 = st.qs[nt][1];
+      const float p0 = fast_exp2(fmaf(sc[nt][0], qs0, mu0)), p1 = fast_exp2(fmaf(sc[nt][1], qs1, mu1));
+      const float p2 = fast_exp2(fmaf(sc[nt][2], qs0, mu0)), p3 = fast_exp2(fmaf(sc[nt][3], qs1, mu1));
       st.l[nt][0] += p0 + p2;
       st.l[nt][1] += p1 + p3;
       // the weights meet V in 16 bits, as in the dense walk; their sum is kept of the unrounded ones

@@ -294,8 +294,9 @@ def paged_sparse_decode(out: torch.Tensor, query: torch.Tensor, key_cache: torch
     and kv head h see only the tokens of `pages[r, h]` (int32 (rows, kv_heads, budget), numbers of the sequence's pages;
     negative entries and pages past the sequence are none) that lie below `seq_lens[r]`. A page listed twice counts
     twice. With nothing left a row answers zeros. `out_lse` (rows, q_heads) fp32 gets the natural-log sum-exp of the
-    scaled scores (-inf for nothing), so that answers over disjoint pages can be merged (`merge_partials`). A NaN among
-    a row's visible keys, or a logit outside fp32's range, makes the heads that meet it NaN."""
+    scaled scores (-inf for nothing), so that answers over disjoint pages can be merged (`merge_partials`). A NaN in a
+    head's query or among its visible keys, or a logit past fp32's greatest, makes the head NaN; one below its lowest is
+    -inf and has no weight. An fp8 cache's query may have any magnitude bf16 has: each head is scaled by a power of two."""
     qshape, qs = _query(query)
     os = out.stride()
     if out.shape != qshape or out.dtype is not query.dtype or os[2] != 1:

@@ -568,7 +568,8 @@ int hkb_select_pages(const hkb_select_pages_t* args, void* stream);
  * entry, or one past the sequence or max_pages, is no page; a page that is listed twice counts twice. A row that is
  * left with nothing answers zeros and, if out_lse (fp32, (rows, q heads)) is not NULL, -inf; otherwise out_lse gets
  * the natural-log sum-exp of the scaled scores, so the answer can be merged with another (hkb_merge). scale and
- * k_scale must be positive. One launch, no scratch. out is 8-byte aligned, with strides that are multiples of 4.
+ * k_scale must be positive. A NaN in a head's query or among its visible keys, or a logit past fp32's greatest, makes the
+ * head NaN. q may have any magnitude: over an fp8 cache each head is multiplied in fp16 after scaling by a power of two. One launch, no scratch. out is 8-byte aligned, with strides that are multiples of 4.
  */
 typedef struct {
   void* out;

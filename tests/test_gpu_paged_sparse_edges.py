@@ -1,13 +1,14 @@
 """Decode over selected pages where its contract is easily broken: refused requests, extreme and infinite values, wide
 strides, the integers' ends, block tables past one chunk of requests, tables wider than every sequence."""
 
+import math
 import random
 
 import pytest
 import torch
 
 from oracle import sparse_oracle as orc
-from test_gpu_paged_sparse import _Loop, _cache_case, _cu, _lens, _ps, _same
+from test_gpu_paged_sparse import (BF, _Loop, _attend, _cache_case, _check_attend, _cu, _lens, _ps, _random_pages, _same)
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +47,45 @@ def test_page_bounds_of_starts_past_the_steps_rows(page, rows):
     _ps().update_page_bounds(b, _cu(c["k"]), _cu(c["table"]), _lens(c), torch.tensor(starts, dtype=torch.int32).cuda(),
                              num_tokens=rows)
     assert _same(b, orc.bounds_ref(b0, c["k"], c["table"], lens, [min(s, rows) for s in starts]))
+
+
+# ------------------------------------------------------------------------------ queries over an fp8 cache
+
+@pytest.mark.parametrize("d, group, power", [(64, 4, 100), (128, 8, -100), (128, 12, 17), (256, 16, 100), (256, 3, -40)])
+def test_fp8_attention_takes_queries_of_any_magnitude(d, group, power):
+    """A power of two moved from the scale to the query changes no logit, and so no bit of the answer."""
+    c = _cache_case([200, 1, 33], d=d, h_kv=2, group=group, kv="fp8", seed=d + group)
+    pages = _random_pages(c, 6)
+    want, lse = _attend(c, pages)
+    _check_attend(c, pages, want, lse)
+    c.update(q=(c["q"].float() * 2.0 ** power).to(BF), scale=c["scale"] * 2.0 ** -power)
+    got, lse_p = _attend(c, pages)
+    assert torch.equal(got, want) and torch.equal(lse_p, lse)
+
+
+@pytest.mark.parametrize("d, group", [(64, 4), (128, 12), (256, 8)])
+def test_fp8_attention_scales_every_head_by_itself(d, group):
+    """Heads of one kv head between 2^-9 and 2^18, past fp16's 65504: logits up to some hundreds, as the oracle has them."""
+    c = _cache_case([300, 17], d=d, h_kv=1, group=group, kv="fp8", seed=d)
+    size = 2.0 ** torch.linspace(-9, 18, group)
+    c.update(q=(c["q"].float() * size[None, :, None]).to(BF), scale=c["scale"] * 2.0 ** -10)
+    assert float(c["q"].float().abs().max()) > 2 * 65504
+    pages = _random_pages(c, 9)
+    got, lse = _attend(c, pages)
+    _check_attend(c, pages, got, lse)
+
+
+@pytest.mark.parametrize("d, group", [(64, 4), (128, 12), (256, 8)])
+def test_fp8_attention_shows_a_broken_query(d, group):
+    """A NaN or infinite element makes its own head NaN (an infinite logit of either sign is among the keys') and no other."""
+    c = _cache_case([300, 90, 40], d=d, h_kv=2, group=group, kv="fp8", seed=d)
+    pages = _random_pages(c, 9)
+    want, lse = _attend(c, pages)
+    heads = c["q"].shape[1]
+    bad = torch.zeros(3, heads, dtype=torch.bool)
+    for r, (h, x) in enumerate([(1, math.nan), (heads - 1, math.inf), (group - 1, -math.inf)]):
+        c["q"][r, h, 5 * r + 3] = x
+        bad[r, h] = True
+    got, lse_b = _attend(c, pages)
+    assert torch.isnan(got[bad.cuda()]).all() and torch.isnan(lse_b[bad.cuda()]).all()
+    assert torch.equal(got[~bad.cuda()], want[~bad.cuda()]) and torch.equal(lse_b[~bad.cuda()], lse[~bad.cuda()])
