@@ -75,7 +75,7 @@ struct TileLoader {
   int tiles_per_page, num_blocks;
   // per-lane constants (set by `prepare`): where this lane's chunk sits in a row group
   uint32_t dst[NPAT];    // shared-memory offset of iteration q (mod NPAT), without it * 512
-  int lane_k, lane_v;    // global offset of the lane's chunk in iteration 0
+  int64_t lane_k, lane_v;   // global offset of the lane's chunk in iteration 0
   bool k_flat, v_flat;   // the 16 rows of a tile are contiguous in global memory
 
   __device__ __forceinline__ void prepare(int lane) {
@@ -83,13 +83,13 @@ struct TileLoader {
 #pragma unroll
     for (int q = 0; q < NPAT; ++q)
       dst[q] = UNIT32 ? tile_off_f8<UNIT32 ? ROWB : 128>(RPI * q + rl, c) - RPI * q * ROWB : tile_off<ROWB>(RPI * q + rl, c) - RPI * q * ROWB;
-    lane_k = rl * (int)kst + c * 16;
-    lane_v = rl * (int)vst + c * 16;
+    lane_k = rl * kst + c * 16;
+    lane_v = rl * vst + c * 16;
     k_flat = kst == ROWB;
     v_flat = vst == ROWB;
   }
 
-  __device__ __forceinline__ void copy_tile(uint32_t smem_tile, const uint8_t* p, int64_t st, int lane_off,
+  __device__ __forceinline__ void copy_tile(uint32_t smem_tile, const uint8_t* p, int64_t st, int64_t lane_off,
                                             bool flat) const {
     p += lane_off;
     if (flat) {   // iteration it is 512 bytes on: immediates

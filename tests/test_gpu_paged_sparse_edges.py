@@ -7,8 +7,10 @@ import random
 import pytest
 import torch
 
+from oracle import paged_oracle as dense
 from oracle import sparse_oracle as orc
-from test_gpu_paged_sparse import (BF, _Loop, _attend, _cache_case, _check_attend, _cu, _lens, _ps, _random_pages, _same)
+from test_gpu_paged_sparse import (BF, _Loop, _attend, _cache_case, _check_attend, _cu, _hold, _lens, _ps, _random_pages,
+                                   _same)
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +91,41 @@ def test_fp8_attention_shows_a_broken_query(d, group):
     got, lse_b = _attend(c, pages)
     assert torch.isnan(got[bad.cuda()]).all() and torch.isnan(lse_b[bad.cuda()]).all()
     assert torch.equal(got[~bad.cuda()], want[~bad.cuda()]) and torch.equal(lse_b[~bad.cuda()], lse[~bad.cuda()])
+
+
+# ------------------------------------------------------------------------------ wide strides
+
+def test_a_cache_whose_tokens_lie_hundreds_of_megabytes_apart():
+    """Token-major across the whole pool, K and V side by side: seven tokens are more than 2^31 bytes."""
+    from hk_dsl_b200.ops import paged
+    nb, page, d = 2_400_000, 16, 64
+    assert 7 * nb * 2 * d > 2 ** 31
+    store = torch.empty(page, nb, 2, 1, d, dtype=torch.uint8, device="cuda")
+    k8, v8 = store[:, :, 0].transpose(0, 1), store[:, :, 1].transpose(0, 1)
+    ids = torch.tensor([[nb - 1, 0, nb // 2, nb - 2, 77], [5, nb // 3, 0, 0, 0]], dtype=torch.int32)
+    lens, ks = [5 * page - 3, page + 1], torch.tensor([0.0125])
+    g = torch.Generator().manual_seed(3)
+    raw = dense.quantize_fp8(torch.randn(2, 10, page, 1, d, generator=g), ks)
+    at = ids.flatten().unique()                # a page of its own for each id, the rest of the pool as it was
+    k, v = raw[0, :at.numel()].view(torch.uint8), raw[1, :at.numel()].view(torch.uint8)
+    for i, b in enumerate(at.tolist()):
+        k8[b], v8[b] = k[i].cuda(), v[i].cuda()
+    small = torch.searchsorted(at, ids).to(torch.int32)
+    q = torch.randn(2, 8, d, generator=g).to(BF)
+    pages = torch.tensor([[0, 2, 4], [0, 1, -1]], dtype=torch.int32).view(2, 1, 3)
+    cu = lambda x: x.cuda()  # noqa: E731
+    n = torch.tensor(lens, dtype=torch.int32).cuda()
+
+    out, lse = torch.empty(2, 8, d, dtype=BF, device="cuda"), torch.empty(2, 8, device="cuda")
+    _ps().paged_sparse_decode(out, cu(q), k8, v8, cu(ids), n, cu(pages), d ** -0.5, "fp8", cu(ks), cu(ks), out_lse=lse)
+    want, tol, wl, tl = orc.sparse_ref(q, k, v, small, lens, pages, d ** -0.5, ks, ks)
+    _hold(out, want, tol)
+    _hold(lse, wl, tl)
+    every = torch.arange(5, dtype=torch.int32).expand(2, 1, 5)
+    paged.paged_attention_decode(out, cu(q), k8, v8, cu(ids), n, d ** -0.5, "fp8", cu(ks), cu(ks))
+    want, tol, _, _ = orc.sparse_ref(q, k, v, small, lens, every, d ** -0.5, ks, ks)
+    _hold(out, want, tol)
+    bounds = torch.zeros(nb, 1, 2, d, dtype=torch.uint8, device="cuda")
+    _ps().update_page_bounds(bounds, k8, cu(ids), n, cu(torch.tensor([0, lens[0], sum(lens)], dtype=torch.int32)), num_tokens=sum(lens))
+    want = orc.bounds_ref(torch.zeros(at.numel(), 1, 2, d, dtype=torch.uint8), k, small, lens, [0, lens[0], sum(lens)])
+    assert _same(bounds[at.long().cuda()], want)
