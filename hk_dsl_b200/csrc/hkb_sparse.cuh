@@ -38,7 +38,8 @@ struct SparseWorker {
   // As the walk's, but for an fp8 cache's query, which the walk cuts at f16's range: here each head is scaled into it, and
   // NaN and infinities stay what they are.
   __device__ static __forceinline__ void begin(State& st, const DecodeArgs& a, int row, int hq0, int nh, int lane, float qs) {
-    Walk::begin(st, a, row, hq0, nh, lane, qs);
+    if constexpr (FP8) Walk::clear(st, lane);
+    else Walk::begin(st, a, row, hq0, nh, lane, qs);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       st.qs[nt][0] = st.qs[nt][1] = qs;

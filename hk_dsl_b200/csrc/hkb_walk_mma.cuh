@@ -519,8 +519,8 @@ struct WalkMMAF8 {
     uint32_t koff[SPANS], voff[SPANS][2];   // this lane's byte offsets inside a K tile / a V tile
   };
 
-  __device__ static __forceinline__ void begin(State& st, const DecodeArgs& a, int row, int hq0, int nh, int lane,
-                                               float /*qs*/) {
+  // The state but for the queries.
+  __device__ static __forceinline__ void clear(State& st, int lane) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int s = 0; s < SPANS; ++s) {
@@ -528,6 +528,21 @@ struct WalkMMAF8 {
       st.voff[s][0] = tile_off_f8<ROWB>(2 * t, 2 * s + (g >> 2)) + (g & 3) * 4;
       st.voff[s][1] = tile_off_f8<ROWB>(2 * t + 1, 2 * s + (g >> 2)) + (g & 3) * 4;
     }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int kc = 0; kc < KD; ++kc)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.o[nt][kc][i] = 0.f;
+      st.m[nt][0] = st.m[nt][1] = -INFINITY;
+      st.l[nt][0] = st.l[nt][1] = 0.f;
+    }
+  }
+
+  __device__ static __forceinline__ void begin(State& st, const DecodeArgs& a, int row, int hq0, int nh, int lane,
+                                               float /*qs*/) {
+    const int g = lane >> 2, t = lane & 3;
+    clear(st, lane);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int h = nt * 8 + g;
@@ -544,12 +559,6 @@ struct WalkMMAF8 {
         st.qb[nt][2 * s][0] = f[0]; st.qb[nt][2 * s][1] = f[1];
         st.qb[nt][2 * s + 1][0] = f[2]; st.qb[nt][2 * s + 1][1] = f[3];
       }
-#pragma unroll
-      for (int kc = 0; kc < KD; ++kc)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) st.o[nt][kc][i] = 0.f;
-      st.m[nt][0] = st.m[nt][1] = -INFINITY;
-      st.l[nt][0] = st.l[nt][1] = 0.f;
     }
   }
 
