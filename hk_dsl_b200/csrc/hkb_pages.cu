@@ -515,6 +515,31 @@ __device__ __forceinline__ float max_nan(float x, float y) {
   return r;
 }
 
+// A page's best product from the definition, by one warp: max_g sum_d max(q_gd low_d, q_gd high_d) for 16-bit summaries.
+// Of an infinite bound only the product that counts is in it. `q`: the group's first head; `low`: the page's summary.
+template <int KIND, int D>
+__device__ __forceinline__ float score_by_definition(const __nv_bfloat16* q, int64_t q_stride_head, int group, const uint8_t* low, int lane) {
+  auto wide = [](uint32_t x) {
+    return KIND == HKB_KV_F16 ? __half22float2(*reinterpret_cast<__half2*>(&x)) : make_float2(bf16lo(x), bf16hi(x));
+  };
+  float best = -INFINITY;
+#pragma unroll 1
+  for (int h = 0; h < group; ++h) {
+    float s = 0.f;
+#pragma unroll 1
+    for (int d = lane * 2; d < D; d += 64) {
+      const float2 x = wide(__ldg(reinterpret_cast<const uint32_t*>(q + (int64_t)h * q_stride_head + d)));
+      const float2 a = wide(__ldg(reinterpret_cast<const uint32_t*>(low + d * 2)));
+      const float2 b = wide(__ldg(reinterpret_cast<const uint32_t*>(low + (D + d) * 2)));
+      s += max_nan(x.x * a.x, x.x * b.x) + max_nan(x.y * a.y, x.y * b.y);
+    }
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+    best = max_nan(best, s);
+  }
+  return best;
+}
+
 template <int KIND, int D, int NT>
 __global__ void __launch_bounds__(SCORE_WARPS * 32, 8) scores_kernel(const ScoreArgs a) {
   constexpr bool FP8 = KIND == HKB_KV_FP8_E4M3, F16 = KIND != HKB_KV_BF16;   // e4m3 widens to f16 exactly
@@ -664,7 +689,20 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32, 8) scores_kernel(const Score
       best[j] = max_nan(best[j], __shfl_xor_sync(0xffffffffu, best[j], 2));
     }
     const int p = p0 + g + 8 * (t & 1);
-    if (t < 2 && p < end) out[p] = (t ? best[1] : best[0]) * factor;
+    float mine = t & 1 ? best[1] : best[0];
+    if constexpr (!FP8) {
+      // The rewritten product meets the half of the wrong sign with a zero, and of an infinite bound that is NaN though
+      // max(q low, q high) may be finite: pages without a number are computed again. (e4m3 has no infinities.)
+      for (unsigned bad = __ballot_sync(0xffffffffu, t < 2 && p < end && mine != mine); bad; bad &= bad - 1) {
+        const int from = __ffs(bad) - 1;
+        const int id = __ldg(table + __shfl_sync(0xffffffffu, p, from));
+        const uint8_t* low = a.bounds + (int64_t)min(max(id, 0), a.num_blocks - 1) * a.b_stride_block + (int64_t)head * a.b_stride_head;
+        const float again = score_by_definition<KIND, D>(
+            a.q + (int64_t)row * a.q_stride_row + (int64_t)(head * a.group) * a.q_stride_head, a.q_stride_head, a.group, low, lane);
+        if (lane == from) mine = again;
+      }
+    }
+    if (t < 2 && p < end) out[p] = mine * factor;
   }
   cp_async_wait<0>();
 }

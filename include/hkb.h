@@ -524,9 +524,10 @@ int hkb_page_bounds(const hkb_page_bounds_t* args, void* stream);
 /*
  * Page scores: scores[r, h, p] = scale * k_scale * max over the query heads g of kv head h of
  * sum_d max(q[r, g, d] * low_d, q[r, g, d] * high_d), low and high from page block_table[r, p]'s summary: no key
- * between them has a greater logit. Computed as max(q, 0) . high + min(q, 0) . low in fp32 (an infinite bound that
- * meets a zero gives NaN). Pages at or past ceil(seq_lens[r] / block_size) get -inf, in all num_columns columns of
- * the table. A NaN among a page's products makes its score NaN. q is bf16 (fp16 with HKB_KV_F16); scores fp32 with
+ * between them has a greater logit. Sums in fp32. An infinite bound counts where its product is the greater one; it gives
+ * NaN where the query is zero, and where both infinities are added. Pages at or past ceil(seq_lens[r] / block_size) get
+ * -inf, in all num_columns columns of the table. A NaN among a page's products makes its score NaN. q is bf16 (fp16 with
+ * HKB_KV_F16); scores fp32 with
  * contiguous columns; k_scale as in hkb_paged_decode.
  */
 typedef struct {

@@ -123,9 +123,11 @@ def scores_ref(q, bounds, table, lens, page, scale, k_scale=None):
             lo, hi = b64[int(table[r, p].clamp(0, bounds.shape[0] - 1))].unbind(1)     # (kv heads, D)
             for h in range(hkv):
                 qq = q64[r, h * g:(h + 1) * g]
-                out[r, h, p] = (qq.clamp(min=0) @ hi[h] + qq.clamp(max=0) @ lo[h]).amax() * unit
-                mag = (qq.abs() * torch.maximum(lo[h].abs(), hi[h].abs())).sum(-1).amax()
-                small = 2.0 ** -38 * qq.abs().amax() * (lo[h].abs() + hi[h].abs()).sum() if k_scale is not None else 0.0
+                out[r, h, p] = torch.maximum(qq * lo[h], qq * hi[h]).sum(-1).amax() * unit
+                # an infinite bound is no part of a finite score, and so of none of its sums
+                al, ah = (torch.where(torch.isinf(x[h]), 0.0, x[h].abs()) for x in (lo, hi))
+                mag = (qq.abs() * torch.maximum(al, ah)).sum(-1).amax()
+                small = 2.0 ** -38 * qq.abs().amax() * (al + ah).sum() if k_scale is not None else 0.0
                 tol[r, h, p] = unit * (mag * (2 * d + 4) * 2.0 ** -23 + small)
     return out, tol
 

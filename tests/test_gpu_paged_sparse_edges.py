@@ -9,8 +9,8 @@ import torch
 
 from oracle import paged_oracle as dense
 from oracle import sparse_oracle as orc
-from test_gpu_paged_sparse import (BF, _Loop, _attend, _cache_case, _check_attend, _cu, _hold, _lens, _ps, _random_pages,
-                                   _same)
+from test_gpu_paged_sparse import (BF, _Loop, _attend, _bounds_of, _cache_case, _check_attend, _cu, _hold, _lens, _ps,
+                                   _random_pages, _same)
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +129,34 @@ def test_a_cache_whose_tokens_lie_hundreds_of_megabytes_apart():
     _ps().update_page_bounds(bounds, k8, cu(ids), n, cu(torch.tensor([0, lens[0], sum(lens)], dtype=torch.int32)), num_tokens=sum(lens))
     want = orc.bounds_ref(torch.zeros(at.numel(), 1, 2, d, dtype=torch.uint8), k, small, lens, [0, lens[0], sum(lens)])
     assert _same(bounds[at.long().cuda()], want)
+
+
+# ------------------------------------------------------------------------------ infinite summaries
+
+@pytest.mark.parametrize("kv", ["bf16", "f16"])
+@pytest.mark.parametrize("d, group", [(64, 1), (64, 4), (128, 8), (128, 12), (256, 5), (256, 16)])
+def test_page_scores_of_infinite_bounds_are_the_definitions(kv, d, group):
+    """max(q low, q high) is finite where the infinite bound is the lesser of the two products; a query of zero that meets an
+    infinity is no number, and neither is a sum of both infinities."""
+    c = _cache_case([16 * 39 + 5, 16 * 3], d=d, h_kv=2, group=group, kv=kv, seed=d + group)
+    b = _bounds_of(c)
+    g = torch.Generator().manual_seed(group)
+    for p in range(39):                      # pages 20 to 23 and the last one keep finite bounds
+        if p in (20, 21, 22, 23):
+            continue
+        for _ in range(1 + p % 3):
+            h, x = int(torch.randint(2, (), generator=g)), int(torch.randint(d, (), generator=g))
+            kind = p % 5
+            low, high = b[int(c["table"][0, p]), h, :, x]
+            b[int(c["table"][0, p]), h, :, x] = torch.tensor(
+                [[float(low), math.inf], [-math.inf, float(high)], [-math.inf, math.inf], [math.inf, math.inf], [-math.inf, -math.inf]][kind])
+    c["q"][0, 0, ::7] = 0.0
+    c["q"][0, group, 1::7] = -0.0
+    want, tol = orc.scores_ref(c["q"], b, c["table"], c["lens"], 16, c["scale"])
+    fin = torch.isfinite(want[0, :, :39])
+    assert 20 < int(fin.sum()) < 78 and torch.isfinite(tol[0, :, :39][fin]).all()
+    got = torch.full(want.shape, 5.0, device="cuda")
+    _ps().page_scores(got, c["q"].cuda(), b.cuda(), c["table"].cuda(), _lens(c), c["scale"], 16)
+    got = got.cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isposinf(got), torch.isposinf(want))
+    _hold(got, want, tol)
