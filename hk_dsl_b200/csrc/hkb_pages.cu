@@ -279,8 +279,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) advance_kernel(const AdvanceArg
       if (!once) adv_chunk(a, c, c0, count, at, total, q);
       const int64_t at0 = count - taken + at.give;
       const int pages = clamp31(min((int64_t)total.give, a.free_cap - at0));
-      for (int x = rank * THREADS + tid; x < pages; x += ctas * THREADS) {
-        const int i = range_of(c.gives, 0, n, x);           // its last pages, gives[i] - x of them from here
+      for (int64_t y = rank * THREADS + tid; y < pages; y += ctas * THREADS) {      // `pages` may be 2^31 - 1
+        const int x = (int)y, i = range_of(c.gives, 0, n, x);                       // its last pages, gives[i] - x of them from here
         a.free_pages[at0 + x] = a.table[(int64_t)(c0 + i) * a.table_stride + c.have[i] - (c.gives[i] - x)];
       }
       at = at + total;
@@ -1005,6 +1005,9 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectArgs a) {
   }
 }
 
+// What a kernel's 32-bit counter runs up to, in steps of less than as much again.
+constexpr int COUNTER_MAX = 1 << 30;
+
 // More than 48 KB of dynamic shared memory, or a cluster past the portable size, is asked for once a device.
 template <class K>
 static cudaError_t arm(K kernel, cudaFuncAttribute attribute, int value, bool (&armed)[64]) {
@@ -1066,7 +1069,7 @@ static int page_bounds(void* bounds, int64_t bounds_stride_block, int64_t bounds
   if (num_seqs == 0 || max_pages == 0) return HKB_OK;
   if (!bounds || !kc.ptr || !block_table || !seq_lens) return HKB_ERR_NULL;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return HKB_ERR_HEAD_DIM;
-  if (block_size <= 0) return HKB_ERR_BLOCK_SIZE;
+  if (block_size <= 0 || block_size > COUNTER_MAX) return HKB_ERR_BLOCK_SIZE;
   if (kv_dtype != HKB_KV_BF16 && kv_dtype != HKB_KV_FP8_E4M3 && kv_dtype != HKB_KV_F16) return HKB_ERR_DTYPE;
   const int es = kv_dtype == HKB_KV_FP8_E4M3 ? 1 : 2;
   if ((kc.stride_block | kc.stride_token | kc.stride_head | bounds_stride_block | bounds_stride_head) * es % 16) return HKB_ERR_STRIDE;
@@ -1109,7 +1112,8 @@ static int page_scores(float* scores, int64_t scores_stride_row, int64_t scores_
                                int64_t bounds_blocks, const int32_t* block_table, int64_t table_stride,
                                const int32_t* seq_lens, int num_rows, int num_q_heads, int num_kv_heads, int head_dim,
                                int block_size, float scale, int kv_dtype, const float* k_scale, void* stream) {
-  if (num_rows < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_columns < 0 || num_rows > 65535 || num_kv_heads > 65535) return HKB_ERR_SIZE;
+  if (num_rows < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_columns < 0 || num_columns > COUNTER_MAX ||
+      num_rows > 65535 || num_kv_heads > 65535) return HKB_ERR_SIZE;
   if (num_rows == 0 || num_columns == 0) return HKB_OK;
   if (!scores || !q || !bounds || !block_table || !seq_lens) return HKB_ERR_NULL;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return HKB_ERR_HEAD_DIM;
@@ -1154,8 +1158,8 @@ static int select_pages(int32_t* pages, int64_t pages_stride_row, int64_t pages_
                                 const float* scores, int64_t scores_stride_row, int64_t scores_stride_head, int num_columns,
                                 const int32_t* seq_lens, int num_rows, int num_kv_heads, int block_size, int first, int last,
                                 void* stream) {
-  if (num_rows < 0 || num_kv_heads <= 0 || num_kv_heads > 65535 || num_columns < 0 || budget < 0 || first < 0 || last < 0 ||
-      (int64_t)first + last > budget) return HKB_ERR_SIZE;
+  if (num_rows < 0 || num_kv_heads <= 0 || num_kv_heads > 65535 || num_columns < 0 || num_columns > COUNTER_MAX ||
+      budget < 0 || budget > COUNTER_MAX || first < 0 || last < 0 || (int64_t)first + last > budget) return HKB_ERR_SIZE;
   if (num_rows == 0 || budget == 0) return HKB_OK;
   if (block_size <= 0) return HKB_ERR_BLOCK_SIZE;
   if (!pages || !seq_lens || (num_columns > 0 && !scores)) return HKB_ERR_NULL;

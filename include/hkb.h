@@ -455,7 +455,8 @@ int hkb_paged_decode_static(void* out, int64_t out_stride_tok, int64_t out_strid
  * Decode over selected pages, and the page bookkeeping under it. These calls are made a handful a layer and take a few
  * microseconds on the GPU, and they have many arguments, so each takes them in one struct (read before it returns) whose
  * every field is eight bytes: a binder fills it as one array of 64-bit words. (From Python, 28 arguments by ctypes
- * cost 2.6 us a call, the packed struct 0.6.) Counts and sizes must fit an int, except where a field says otherwise.
+ * cost 2.6 us a call, the packed struct 0.6.) Counts and sizes must fit an int, except where a field says otherwise;
+ * the columns of scores, a selection's budget and the page size of a summary are 2^30 at most.
  */
 
 /*

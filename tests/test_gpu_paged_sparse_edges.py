@@ -9,8 +9,8 @@ import torch
 
 from oracle import paged_oracle as dense
 from oracle import sparse_oracle as orc
-from test_gpu_paged_sparse import (BF, _Loop, _attend, _bounds_of, _cache_case, _check_attend, _cu, _hold, _lens, _ps,
-                                   _random_pages, _same)
+from test_gpu_paged_sparse import (BF, _Loop, _attend, _bounds_of, _cache_case, _check_attend, _cu, _hold, _lens,
+                                   _ps, _random_pages, _same)
 
 pytestmark = pytest.mark.gpu
 
@@ -160,3 +160,19 @@ def test_page_scores_of_infinite_bounds_are_the_definitions(kv, d, group):
     got = got.cpu()
     assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isposinf(got), torch.isposinf(want))
     _hold(got, want, tol)
+
+
+# ------------------------------------------------------------------------------ the integers' ends
+
+def test_advance_tables_takes_back_as_many_pages_as_an_int_counts():
+    """One request gives back 2^31 - 1 pages of one token."""
+    n = 2 ** 31 - 1
+    table = torch.arange(n - 1, -1, -1, dtype=torch.int32, device="cuda").view(1, n)
+    free = torch.full((n,), -5, dtype=torch.int32, device="cuda")
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    lens, count, starts, status = i32(n), i32(0), i32(7, 7), i32(7)
+    slots = torch.full((1,), 7, dtype=torch.int64, device="cuda")
+    pos = slots.clone()
+    _ps().advance_tables(table, lens, i32(-n), free, count, 1, slots, pos, starts, status)
+    assert int(lens) == 0 and int(count) == n and int(status) == orc.OK and int(slots) == -1 and starts.tolist() == [0, 0]
+    assert torch.equal(free, table[0])
