@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(WARPS * 32, sparse_ctas<P, WARPS>()) sparse_ke
     cp_async_wait<NST - 2>();
     __syncwarp();
     const int t = issue(sl);     // over the tile before
-    P::step(st, ring + sc * P::STAGE_BYTES, queue[0], seq_len, queue[0] + TILE_TOKENS > seq_len, lane);
+    P::step(st, ring + sc * P::STAGE_BYTES, queue[0], seq_len, queue[0] > seq_len - TILE_TOKENS, lane);
 #pragma unroll
     for (int k = 0; k + 1 < NST - 1; ++k) queue[k] = queue[k + 1];
     queue[NST - 2] = t;

@@ -176,3 +176,21 @@ def test_advance_tables_takes_back_as_many_pages_as_an_int_counts():
     _ps().advance_tables(table, lens, i32(-n), free, count, 1, slots, pos, starts, status)
     assert int(lens) == 0 and int(count) == n and int(status) == orc.OK and int(slots) == -1 and starts.tolist() == [0, 0]
     assert torch.equal(free, table[0])
+
+
+def test_paged_sparse_decode_of_a_sequence_that_ends_where_ints_do():
+    """The tile of positions 2^31 - 16 .. 2^31 - 1 holds 15 tokens of a sequence of 2^31 - 1; the last one is nobody's."""
+    page, d, last = 16, 64, 2 ** 27 - 1
+    g = torch.Generator().manual_seed(1)
+    k, v = torch.randn(3, page, 1, d, generator=g).to(BF), torch.randn(3, page, 1, d, generator=g).to(BF)
+    k[2, 15] = v[2, 15] = math.nan
+    q = torch.randn(1, 4, d, generator=g).to(BF)
+    table = torch.zeros(1, last + 1, dtype=torch.int32, device="cuda")
+    table[0, last], table[0, last - 1] = 2, 1
+    pages = torch.tensor([0, last - 1, last], dtype=torch.int32).view(1, 1, 3)
+    out, lse = torch.empty(1, 4, d, dtype=BF, device="cuda"), torch.empty(1, 4, device="cuda")
+    _ps().paged_sparse_decode(out, q.cuda(), k.cuda(), v.cuda(), table, torch.tensor([2 ** 31 - 1], dtype=torch.int32).cuda(),
+                              pages.cuda(), d ** -0.5, out_lse=lse)
+    want, tol, wl, tl = orc.sparse_ref(q, k, v, torch.tensor([[0, 1, 2]]), [47], torch.arange(3).view(1, 1, 3), d ** -0.5)
+    _hold(out, want, tol)
+    _hold(lse, wl, tl)
