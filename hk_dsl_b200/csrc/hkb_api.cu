@@ -92,7 +92,7 @@ extern "C" const char* hkb_strerror(int code) {
     case HKB_ERR_ALIGN: return "a base pointer is not aligned as the kernels read it";
     case HKB_ERR_SPLITS: return "num_splits out of range, or split scratch missing";
     case HKB_ERR_SIZE: return "a count is negative or past a launch limit";
-    case HKB_ERR_SCALE: return "an fp8 cache needs k_scale and v_scale";
+    case HKB_ERR_SCALE: return "an fp8 cache needs k_scale and v_scale, a softmax scale is positive (2^-126 to 2^126)";
     case HKB_ERR_UNSUPPORTED: return "no kernel for this combination of head_dim, dtype and group";
     case HKB_ERR_STATIC_SCRATCH:
       return "the split partials need more than the library's built-in scratch (HKB_STATIC_SCRATCH_BYTES): use fewer "

@@ -50,6 +50,10 @@ inline bool ints(std::initializer_list<int64_t> values) {
   return true;
 }
 
+// Whether a softmax scale is positive and, in fp32 and times log2 e, neither subnormal nor infinite: at 0 a masked logit,
+// -inf, is no number, and at infinity a logit of 0.
+inline bool positive_scale(double scale) { return scale >= 0x1p-126 && scale <= 0x1p126; }
+
 // The calls of a decode step are short kernels that each read what the one before wrote. They are launched with
 // programmatic stream serialisation: a kernel's CTAs may take their places while the kernel before still runs. Every
 // kernel launched so begins with `after_the_last`, which waits until everything before it is complete and its writes are

@@ -1121,7 +1121,7 @@ static int page_scores(float* scores, int64_t scores_stride_row, int64_t scores_
   if (num_q_heads % num_kv_heads || num_q_heads / num_kv_heads > HKB_MAX_GROUP) return HKB_ERR_GROUP;
   if (kv_dtype != HKB_KV_BF16 && kv_dtype != HKB_KV_FP8_E4M3 && kv_dtype != HKB_KV_F16) return HKB_ERR_DTYPE;
   const bool fp8 = kv_dtype == HKB_KV_FP8_E4M3;
-  if (fp8 && !k_scale) return HKB_ERR_SCALE;
+  if ((fp8 && !k_scale) || !positive_scale(scale)) return HKB_ERR_SCALE;
   const int es = fp8 ? 1 : 2;
   if ((bounds_stride_block | bounds_stride_head) * es % 16 || (q_stride_row | q_stride_head) % 8) return HKB_ERR_STRIDE;
   if (((uintptr_t)q | (uintptr_t)bounds) % 16 || (uintptr_t)scores % 4) return HKB_ERR_ALIGN;

@@ -280,7 +280,7 @@ static int sparse_decode(void* out, int64_t out_stride_tok, int64_t out_stride_h
   if (num_q_heads % num_kv_heads || num_q_heads / num_kv_heads > HKB_MAX_GROUP) return HKB_ERR_GROUP;
   if (kv_dtype != HKB_KV_BF16 && kv_dtype != HKB_KV_FP8_E4M3 && kv_dtype != HKB_KV_F16) return HKB_ERR_DTYPE;
   const bool fp8 = kv_dtype == HKB_KV_FP8_E4M3;
-  if (fp8 && (!k_scale || !v_scale)) return HKB_ERR_SCALE;
+  if ((fp8 && (!k_scale || !v_scale)) || !positive_scale(scale)) return HKB_ERR_SCALE;
   if (kc.num_blocks < 1 || vc.num_blocks < 1) return HKB_ERR_SIZE;
   if ((int64_t)budget * (block_size / TILE_TOKENS) > 0x7fffffff) return HKB_ERR_SIZE;
   const int es = fp8 ? 1 : 2;

@@ -214,8 +214,9 @@ def _code(kv_cache_dtype: str, cache: torch.Tensor, dtype) -> int:
 
 def _positive(scale: float) -> float:
     scale = float(scale)
-    if not scale > 0.0:
-        raise ValueError(f"{_WHO}: scale {scale}: the greatest logit is only bounded for a positive one")
+    if not 2.0 ** -126 <= scale <= 2.0 ** 126:
+        raise ValueError(f"{_WHO}: scale {scale}: a positive number that fp32 holds in full needed (2^-126 to 2^126); the "
+                         f"greatest logit is only bounded for a positive one")
     return scale
 
 

@@ -55,7 +55,7 @@ typedef enum {
   HKB_ERR_ALIGN = -7,       /* a base pointer is not 16-byte aligned */
   HKB_ERR_SPLITS = -8,      /* num_splits < 1, > HKB_MAX_SPLITS, or scratch missing */
   HKB_ERR_SIZE = -9,        /* a count is negative or a grid limit is exceeded */
-  HKB_ERR_SCALE = -10,      /* fp8 cache without k_scale / v_scale */
+  HKB_ERR_SCALE = -10,      /* fp8 cache without k_scale / v_scale; a scale outside [2^-126, 2^126] where a call needs it positive */
   HKB_ERR_UNSUPPORTED = -11,/* a combination this build has no kernel for */
   HKB_ERR_STATIC_SCRATCH = -12, /* the split partials would not fit the library's built-in scratch */
   HKB_ERR_CUDA = -100       /* CUDA reported an error at launch (see hkb_last_cuda_error) */
@@ -525,11 +525,11 @@ int hkb_page_bounds(const hkb_page_bounds_t* args, void* stream);
 /*
  * Page scores: scores[r, h, p] = scale * k_scale * max over the query heads g of kv head h of
  * sum_d max(q[r, g, d] * low_d, q[r, g, d] * high_d), low and high from page block_table[r, p]'s summary: no key
- * between them has a greater logit. Sums in fp32. An infinite bound counts where its product is the greater one; it gives
- * NaN where the query is zero, and where both infinities are added. Pages at or past ceil(seq_lens[r] / block_size) get
- * -inf, in all num_columns columns of the table. A NaN among a page's products makes its score NaN. q is bf16 (fp16 with
- * HKB_KV_F16); scores fp32 with
- * contiguous columns; k_scale as in hkb_paged_decode.
+ * between them has a greater logit. scale lies in [2^-126, 2^126], k_scale is positive. Sums in fp32. An infinite bound
+ * counts where its product is the greater one; it gives NaN where the query is zero, and where both infinities are added.
+ * Pages at or past ceil(seq_lens[r] / block_size) get -inf, in all num_columns columns of the table. A NaN among a page's
+ * products makes its score NaN. q is bf16 (fp16 with HKB_KV_F16); scores fp32 with contiguous columns; k_scale as in
+ * hkb_paged_decode.
  */
 typedef struct {
   float* scores;
@@ -569,9 +569,10 @@ int hkb_select_pages(const hkb_select_pages_t* args, void* stream);
  * sequence (numbers of its block-table row, not page ids), and of those only tokens below seq_lens[r]. A negative
  * entry, or one past the sequence or max_pages, is no page; a page that is listed twice counts twice. A row that is
  * left with nothing answers zeros and, if out_lse (fp32, (rows, q heads)) is not NULL, -inf; otherwise out_lse gets
- * the natural-log sum-exp of the scaled scores, so the answer can be merged with another (hkb_merge). scale and
- * k_scale must be positive. A NaN in a head's query or among its visible keys, or a logit past fp32's greatest, makes the
- * head NaN. q may have any magnitude: over an fp8 cache each head is multiplied in fp16 after scaling by a power of two. One launch, no scratch. out is 8-byte aligned, with strides that are multiples of 4.
+ * the natural-log sum-exp of the scaled scores, so the answer can be merged with another (hkb_merge). scale lies in
+ * [2^-126, 2^126], k_scale is positive. A NaN in a head's query or among its visible keys, or a logit past fp32's
+ * greatest, makes the head NaN. q may have any magnitude: over an fp8 cache each head is multiplied in fp16 after scaling
+ * by a power of two. One launch, no scratch. out is 8-byte aligned, with strides that are multiples of 4.
  */
 typedef struct {
   void* out;
