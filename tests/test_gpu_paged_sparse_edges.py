@@ -9,8 +9,8 @@ import torch
 
 from oracle import paged_oracle as dense
 from oracle import sparse_oracle as orc
-from test_gpu_paged_sparse import (BF, _Loop, _attend, _bounds_of, _cache_case, _check_attend, _cu, _hold, _lens,
-                                   _ps, _random_pages, _same)
+from test_gpu_paged_sparse import (BF, _Loop, _advance, _attend, _bounds_of, _cache_case, _check_attend, _cu, _hold,
+                                   _lens, _ps, _random_pages, _same, _tables_case)
 
 pytestmark = pytest.mark.gpu
 
@@ -194,3 +194,29 @@ def test_paged_sparse_decode_of_a_sequence_that_ends_where_ints_do():
     want, tol, wl, tl = orc.sparse_ref(q, k, v, torch.tensor([[0, 1, 2]]), [47], torch.arange(3).view(1, 1, 3), d ** -0.5)
     _hold(out, want, tol)
     _hold(lse, wl, tl)
+
+
+# ------------------------------------------------------------------------------ requests past one chunk of the scan
+
+@pytest.mark.parametrize("n, page, width, pool, rows, first_short, first_cut", [
+    (2049, 16, 4, 20000, 60000, None, None),       # a second chunk of one request
+    (5000, 16, 6, 7700, 60000, 0, None),           # the free pages run out in the first chunk, and stay out
+    (5000, 16, 6, 40000, 18000, None, 1),          # the rows in the second
+    (6145, 5, 9, 13700, 15000, 1, 2),              # the pages in the second, the rows in the third
+    (34821, 1, 3, 200000, 23000, None, 14),        # more chunks than the cluster has CTAs
+])
+def test_advance_tables_of_many_requests(n, page, width, pool, rows, first_short, first_cut):
+    table, lens, new, free, count, rows = _tables_case(n, n, page, width, pool, rows)
+    chunk = 2048
+    for i in range(0, n, 1024):                    # somebody gives pages back in every chunk
+        lens[i], new[i] = (0, 1) if lens[i] == 0 else (lens[i], -lens[i])
+    want = orc.advance_ref(table, lens, new, free, count, page, rows)
+    status = want[7]
+    if first_short is not None:
+        assert status.index(orc.NO_PAGES) // chunk == first_short
+    if first_cut is not None:
+        assert status.index(orc.NO_ROWS) // chunk == first_cut
+    assert all(any(m < 0 < k for m, k in zip(new[c:c + chunk], lens[c:c + chunk])) for c in range(0, n - 1, chunk))
+    got = _advance(table, lens, new, free, count, page, rows)
+    for name, g, w in zip(("table", "lens", "free", "count", "slots", "positions", "starts", "status"), got, want):
+        assert g == w, name
