@@ -220,3 +220,54 @@ def test_advance_tables_of_many_requests(n, page, width, pool, rows, first_short
     got = _advance(table, lens, new, free, count, page, rows)
     for name, g, w in zip(("table", "lens", "free", "count", "slots", "positions", "starts", "status"), got, want):
         assert g == w, name
+
+
+# ------------------------------------------------------------------------------ wide tables, rows of one sequence
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("width", [300, 700, 3000, 17000])
+def test_a_table_far_wider_than_its_sequences(kv, width):
+    """As a captured step has it: scores, selection and attention answer as with a table that just holds them, whatever the
+    spare columns hold."""
+    c = _cache_case([16 * 40, 1, 0, 16 * 9 + 5], d=128, h_kv=2, group=4, kv=kv, seed=width)
+    b, tight = _bounds_of(c), c["table"].shape[1]
+    q, ks, lens = c["q"].cuda(), _cu(c["ks"]), _lens(c)
+    table = torch.full((4, width), 2 ** 31 - 1, dtype=torch.int32)
+    table[:, :tight] = c["table"]
+    answers = []
+    for t in (c["table"], table):
+        scores = torch.full((4, 2, t.shape[1]), 9.0, device="cuda")
+        _ps().page_scores(scores, q, b.cuda(), t.cuda(), lens, c["scale"], 16, c["name"], ks)
+        pages = torch.full((4, 2, 12), 99, dtype=torch.int32, device="cuda")
+        _ps().select_pages(pages, scores, lens, 16, first=1, last=2)
+        out, lse = _attend(c, pages.cpu(), table=t)
+        answers.append((scores, pages, out, lse))
+    (s0, p0, o0, l0), (s1, p1, o1, l1) = answers
+    assert torch.equal(s1[:, :, :tight], s0) and torch.isneginf(s1[:, :, tight:]).all()
+    assert torch.equal(p0.cpu(), orc.select_ref(s0.cpu(), c["lens"], 16, 12, 1, 2))
+    assert torch.equal(p1, p0) and torch.equal(o1, o0) and torch.equal(l1, l0)
+    _check_attend(c, p0.cpu(), o0, l0)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_several_tokens_of_one_sequence(kv):
+    """Drafts: a query row for each of a sequence's last tokens, its table row repeated (by `expand` too), one length each."""
+    c = _cache_case([333, 64], d=64, h_kv=2, group=4, kv=kv, seed=7)
+    b = _bounds_of(c)
+    rows = [(0, 330), (0, 331), (0, 332), (0, 333), (1, 63), (1, 64)]
+    lens = [n for _, n in rows]
+    table = c["table"][[r for r, _ in rows]].contiguous()
+    g = torch.Generator().manual_seed(8)
+    c.update(table=table, lens=lens, q=torch.randn(6, 8, 64, generator=g).to(BF))
+    want, tol = orc.scores_ref(c["q"], b, table, lens, 16, c["scale"], c["ks"])
+    scores = torch.zeros(want.shape, device="cuda")
+    _ps().page_scores(scores, c["q"].cuda(), b.cuda(), table.cuda(), _lens(c), c["scale"], 16, c["name"], _cu(c["ks"]))
+    _hold(scores, want, tol)
+    pages = torch.zeros(6, 2, 9, dtype=torch.int32, device="cuda")
+    _ps().select_pages(pages, scores, _lens(c), 16, first=1, last=2)
+    assert torch.equal(pages.cpu(), orc.select_ref(scores.cpu(), lens, 16, 9, 1, 2))
+    out, lse = _attend(c, pages.cpu())
+    _check_attend(c, pages.cpu(), out, lse)
+    part = dict(c, table=table[:1].cuda().expand(4, -1), lens=lens[:4], q=c["q"][:4])      # a row stride of 0
+    got, _ = _attend(part, pages[:4].cpu())
+    assert torch.equal(got, out[:4])
