@@ -262,7 +262,8 @@ def select_pages(pages: torch.Tensor, scores: torch.Tensor, seq_lens: torch.Tens
                  first: int = 1, last: int = 4) -> torch.Tensor:
     """The budget's best pages: `pages` (rows, kv_heads, budget) int32 gets, in ascending order and -1 behind, the
     `first` and the `last` pages of the row's sequence and then those of the greatest `scores` (rows, kv_heads, columns)
-    fp32, ties to the lowest page, NaN above all numbers. A row with no more pages than the budget gets them all.
+    fp32, ties to the lowest page, NaN above all numbers. A row with no more pages than the budget gets them all. What the
+    columns behind a sequence hold makes no difference.
     The entries number the row's pages (columns of its block table), as `paged_sparse_decode` reads them."""
     pshape, ps, lens = pages.shape, pages.stride(), seq_lens.shape
     if pages.dtype is not _I32 or seq_lens.dtype is not _I32 or len(pshape) != 3 or ps[2] != 1 or seq_lens.stride() != (1,):

@@ -528,7 +528,8 @@ int hkb_page_bounds(const hkb_page_bounds_t* args, void* stream);
  * between them has a greater logit. scale lies in [2^-126, 2^126], k_scale is positive. Sums in fp32. An infinite bound
  * counts where its product is the greater one; it gives NaN where the query is zero, and where both infinities are added.
  * Pages at or past ceil(seq_lens[r] / block_size) get -inf, in all num_columns columns of the table. A NaN among a page's
- * products makes its score NaN. q is bf16 (fp16 with HKB_KV_F16); scores fp32 with contiguous columns; k_scale as in
+ * products makes its score NaN. All num_columns entries of a row's table must be readable; those behind the sequence hold
+ * anything. q is bf16 (fp16 with HKB_KV_F16); scores fp32 with contiguous columns; k_scale as in
  * hkb_paged_decode.
  */
 typedef struct {
@@ -551,7 +552,8 @@ int hkb_page_scores(const hkb_page_scores_t* args, void* stream);
  * The budget's best pages of every (row, kv head). Row r has n = min(ceil(seq_lens[r] / block_size), num_columns)
  * pages; its first `first` and last `last` pages are taken, then those of the greatest scores (ties to the lowest
  * page, NaN above all numbers), min(n, budget) in all. pages[r, h, :] gets them in ascending order, -1 behind.
- * first + last <= budget. Columns at or past n are not read.
+ * first + last <= budget. All num_columns columns must be readable (the scores are asked for beside the length, not
+ * behind it); what those at or past n hold makes no difference.
  */
 typedef struct {
   int32_t* pages;
