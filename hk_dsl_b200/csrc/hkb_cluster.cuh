@@ -66,6 +66,19 @@ __device__ __forceinline__ void let_the_next() { asm volatile("griddepcontrol.la
 // pages: 41.2 against 36.2 us a step).
 constexpr int STEP_CARVEOUT = 100;
 
+// More than 48 KB of dynamic shared memory, or a cluster past the portable size, is asked for once a device.
+template <class K>
+inline cudaError_t arm(K kernel, cudaFuncAttribute attribute, int value, bool (&armed)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev >= 0 && dev < 64 && !armed[dev]) {
+    e = cudaFuncSetAttribute(kernel, attribute, value);
+    if (e == cudaSuccess) armed[dev] = true;
+  }
+  if (e != cudaSuccess) { (void)cudaGetLastError(); hkb_tls_cuda_error = (int)e; }
+  return e;
+}
+
 // One argument struct; `cluster` CTAs of grid.x a cluster (1: none; past 8, the portable size, the kernel has to be
 // allowed to).
 inline int launch(const void* kernel, dim3 grid, int threads, int cluster, int smem_bytes, const void* args, cudaStream_t st, int carveout = STEP_CARVEOUT) {

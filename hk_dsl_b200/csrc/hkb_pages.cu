@@ -1008,19 +1008,6 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const SelectArgs a) {
 // What a kernel's 32-bit counter runs up to, in steps of less than as much again.
 constexpr int COUNTER_MAX = 1 << 30;
 
-// More than 48 KB of dynamic shared memory, or a cluster past the portable size, is asked for once a device.
-template <class K>
-static cudaError_t arm(K kernel, cudaFuncAttribute attribute, int value, bool (&armed)[64]) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && dev >= 0 && dev < 64 && !armed[dev]) {
-    e = cudaFuncSetAttribute(kernel, attribute, value);
-    if (e == cudaSuccess) armed[dev] = true;
-  }
-  if (e != cudaSuccess) { (void)cudaGetLastError(); hkb_tls_cuda_error = (int)e; }
-  return e;
-}
-
 template <int KIND, int D, int NT>
 static int launch_scores(const ScoreArgs& a, dim3 grid, cudaStream_t st) {
   static bool armed[64] = {};

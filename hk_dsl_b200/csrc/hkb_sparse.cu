@@ -233,14 +233,8 @@ static int launch_sparse(const SparseArgs& a, int rows, int splits, cudaStream_t
   using P = SparseWorker<D, KIND, NT, NST>;
   auto kernel = sparse_kernel<P, WARPS, KIND == HKB_KV_F16>;
   constexpr int smem = WARPS * P::RING_SMEM;
-  static bool armed[64] = {};    // more than 48 KB of shared memory: asked for once a device
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && dev >= 0 && dev < 64 && !armed[dev]) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess) armed[dev] = true;
-  }
-  if (e != cudaSuccess) { (void)cudaGetLastError(); hkb_tls_cuda_error = (int)e; return HKB_ERR_CUDA; }
+  static bool armed[64] = {};
+  if (arm(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem, armed) != cudaSuccess) return HKB_ERR_CUDA;
   return launch((const void*)kernel, dim3(splits, a.d.num_kv_heads, rows), WARPS * 32, splits, smem, &a, st);
 }
 
