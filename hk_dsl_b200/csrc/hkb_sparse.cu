@@ -202,8 +202,9 @@ __global__ void __launch_bounds__(WARPS * 32, sparse_ctas<P, WARPS>()) sparse_ke
 // Short lists do not pay for the wider clusters: fp8, 16 x 8 items of 16 pages: 4 CTAs 7.1, 8 8.5; bf16, 8 x 8 of 32: 4
 // CTAs 6.4, 8 7.1; with eight heads they pay for a pair from 2048 channels on: fp8, 64 x 8 items of 8 pages 1 CTA 6.8, 2
 // 8.1; of 16 11.9, 11.2; of 48 25.8, 22.0 (sixteen heads, of 16: 18.7, 23.2: registers). Nor for a cluster at all: its
-// barriers and peers' memory cost 1.2 us, half that with an SM a CTA, and a tile costs a warp 0.33, 0.43, 0.66 us (head
-// size 64, 128, 256, eight heads; twice that sixteen). So one CTA of four warps, where the items are one wave of those
+// barriers and peers' memory cost 1.2 us, half that with an SM a CTA, and a tile costs a warp 0.35, 0.42, 0.62 us (bf16,
+// head size 64, 128, 256, up to eight heads; fp8 0.29, 0.49, 0.65), which the rule takes for 0.33, 0.44, 0.66. (Sixteen
+// heads cost 0.40, 0.52, 0.83; taken for twice the eight, since their registers let two CTAs in instead of three.) So one CTA of four warps, where the items are one wave of those
 // (registers let three in, two with sixteen heads) and the tiles a warp has more of, tiles (1/4 - 1/2c), cost less:
 //   bf16, cluster / four warps: 1 x 8 items of 4 pages 4.3 / 3.6, of 8 4.5 / 4.0, of 32 5.2 / 6.6; 16 x 8 of 8 5.8 / 4.3, of
 //   24 7.2 / 7.1, 32 x 8 of 16 8.9 / 8.2; head size 256, 1 x 8 of 8 5.3 / 5.4, 16 x 8 of 8 7.2 / 6.2
