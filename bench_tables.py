@@ -10,6 +10,8 @@ here is part of the bench line.
                                          where the tensor-memory prefill kernel's cycles go, by role
     python bench_tables.py --attrib      the decode walk with one stage left out: what each stage costs
     python bench_tables.py --sparse      a decode step over selected pages, call by call, beside the dense one
+    python bench_tables.py --sparse-shapes [--kv fp8] [--head-dim 64] [--group 16]
+                                         its attention alone over batches and list lengths
 """
 
 from __future__ import annotations
@@ -576,6 +578,31 @@ def layouts_table(only: str = ""):
     return 0 if same else 1
 
 
+def _graph_us(call, layers):
+    """us of call(layer), from a CUDA graph whose calls go round the layers: median of 7 replays."""
+    import torch
+    for l in range(layers):
+        call(l)
+    torch.cuda.synchronize()
+    reps = max(1, 32 // layers)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for _ in range(reps):
+            for l in range(layers):
+                call(l)
+    g.replay()
+    torch.cuda.synchronize()
+    times = []
+    for _ in range(7):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        g.replay()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) * 1e3 / (reps * layers))
+    return round(statistics.median(times), 2)
+
+
 def sparse_table():
     """One layer's decode step over selected pages (hk_dsl_b200.ops.paged_sparse) -- the newest pages' summaries, scores,
     selection, attention -- beside the dense walk and merge over the same caches: us from CUDA graphs whose calls rotate
@@ -587,28 +614,6 @@ def sparse_table():
 
     dev = torch.device("cuda", 0)
     torch.cuda.set_device(dev)
-
-    def timed(call, layers):
-        for l in range(layers):
-            call(l)
-        torch.cuda.synchronize()
-        reps = max(1, 32 // layers)
-        g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
-            for _ in range(reps):
-                for l in range(layers):
-                    call(l)
-        g.replay()
-        torch.cuda.synchronize()
-        times = []
-        for _ in range(7):
-            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-            a.record()
-            g.replay()
-            b.record()
-            torch.cuda.synchronize()
-            times.append(a.elapsed_time(b) * 1e3 / (reps * layers))
-        return round(statistics.median(times), 2)
 
     for reqs, hq, hkv, ctx, kv, budget in ((1, 32, 8, 32768, "auto", 128), (16, 32, 8, 8192, "auto", 64), (64, 32, 8, 8192, "auto", 64),
                                            (128, 32, 8, 4096, "fp8", 64), (2, 64, 8, 131072, "auto", 256),
@@ -634,14 +639,51 @@ def sparse_table():
             "attention": lambda l: ps.paged_sparse_decode(st.out, st.query, st.k_caches[l], st.v_caches[l], st.block_table,
                                                           st.seq_lens, pages, st.scale, kv, st.k_scale, st.v_scale)}
         row = {"requests": n, "q_heads": hq, "kv_heads": hkv, "context": ctx, "kv": kv, "budget_pages": budget, "layers_rotated": layers}
-        row["dense_us"] = timed(lambda l: paged.paged_attention_decode(
+        row["dense_us"] = _graph_us(lambda l: paged.paged_attention_decode(
             st.out, st.query, st.k_caches[l], st.v_caches[l], st.block_table, st.seq_lens, st.scale, kv, st.k_scale, st.v_scale,
             num_splits=splits, scratch=scratch), layers)
-        row["sparse_step_us"] = timed(lambda l: [c(l) for c in calls.values()], layers)
-        row.update({f"{k}_us": timed(c, layers) for k, c in calls.items()})
+        row["sparse_step_us"] = _graph_us(lambda l: [c(l) for c in calls.values()], layers)
+        row.update({f"{k}_us": _graph_us(c, layers) for k, c in calls.items()})
         print(json.dumps(row), flush=True)
         del st, bounds
         torch.cuda.empty_cache()
+    return 0
+
+
+def sparse_shapes_table(kv, head_dim, group):
+    """hk_dsl_b200.ops.paged_sparse.paged_sparse_decode alone over rows x kv heads and pages a (row, kv head), 16-token pages
+    all of them whole: its floor (bytes at the measured copy rate) and its us from CUDA graphs over three states in turn."""
+    import torch
+
+    import bench
+    from hk_dsl_b200.ops import paged_sparse as ps
+
+    dev = torch.device("cuda", 0)
+    torch.cuda.set_device(dev)
+    gbs, _ = bench.measured_peak()
+    fp8, page, d = kv == "fp8", 16, head_dim
+    one = torch.ones(1, device=dev) if fp8 else None
+    gen = torch.Generator(device=dev).manual_seed(1)
+    for rows, hkv in ((1, 8), (2, 8), (4, 8), (8, 8), (16, 8), (32, 8), (48, 8), (64, 8), (128, 8), (64, 2), (3, 1)):
+        for budget in (4, 8, 16, 32, 64, 256, 1024):
+            blocks = rows * budget
+            if blocks * hkv * page * d > 1 << 28:
+                continue
+            states = []
+            for _ in range(3):
+                k, v = (torch.randn(blocks, hkv, page, d, device=dev, generator=gen).to(
+                    torch.float8_e4m3fn if fp8 else torch.bfloat16).transpose(1, 2) for _ in range(2))
+                q = torch.randn(rows, hkv * group, d, device=dev, generator=gen).bfloat16()
+                table = torch.randperm(blocks, device=dev, generator=gen).to(torch.int32).view(rows, budget)
+                states.append((torch.empty_like(q), q, k, v, table))
+            lens = torch.full((rows,), budget * page, dtype=torch.int32, device=dev)
+            pages = torch.arange(budget, dtype=torch.int32, device=dev).expand(rows, hkv, budget).contiguous()
+            us = _graph_us(lambda l: ps.paged_sparse_decode(*states[l], lens, pages, d ** -0.5, kv, one, one), 3)
+            nbytes = rows * hkv * budget * (page * 2 * d * (1 if fp8 else 2) + 4) + 2 * rows * hkv * group * d * 2
+            print(json.dumps({"kv": kv, "head_dim": d, "group": group, "rows": rows, "kv_heads": hkv, "pages": budget,
+                              "floor_us": round(nbytes / gbs / 1e3, 2), "us": us}), flush=True)
+            del states, k, v
+            torch.cuda.empty_cache()
     return 0
 
 
@@ -653,14 +695,19 @@ def main():
                                                "x-split (a small case for a profiler)")
     ap.add_argument("--prefill-trace", action="store_true", help="cycles by role and phase of the tensor-memory prefill kernel")
     ap.add_argument("--attrib", action="store_true", help="the decode walk with one stage left out: what each stage costs")
-    ap.add_argument("--kv", default="bf16", choices=["bf16", "fp8"], help="with --prefill-trace, or --prefill --case: the cache type")
+    ap.add_argument("--kv", default="bf16", choices=["bf16", "fp8"], help="with --prefill-trace, --prefill --case or --sparse-shapes: the cache type")
+    ap.add_argument("--head-dim", type=int, default=128, choices=[64, 128, 256], help="with --sparse-shapes")
+    ap.add_argument("--group", type=int, default=4, help="with --sparse-shapes: query heads a kv head, up to 16")
     ap.add_argument("--sparse", action="store_true", help="a decode step over selected pages, call by call, beside the dense one")
+    ap.add_argument("--sparse-shapes", action="store_true", help="attention over selected pages alone, over batches and list lengths")
     ap.add_argument("--exchange", action="store_true", help="the KV-split exchange kernels on one GPU (one launch against two)")
     ap.add_argument("--shards", action="store_true", help="one rank's share of c2 over 1/2/4/8 GPUs, on one GPU: the step's fixed costs")
     ap.add_argument("--layouts", action="store_true", help="the decode over the usual and the x-split cache layout")
     args = ap.parse_args()
     if args.sparse:
         return sparse_table()
+    if args.sparse_shapes:
+        return sparse_shapes_table(args.kv, args.head_dim, args.group)
     if args.exchange:
         return exchange_table(args.case)
     if args.shards:

@@ -196,20 +196,21 @@ __global__ void __launch_bounds__(WARPS * 32, sparse_ctas<P, WARPS>()) sparse_ke
 // portable cluster: more only adds waves of them (each costs about 6 us whatever it does), fewer leave a batch of few
 // rows to few warps. Where even eight CTAs of two warps leave half the machine's mma pipes idle and each warp has more
 // than eight tiles to go, four warps a CTA. Measured at head size 128, 16-token pages, us:
-//   bf16, 64 x 8 items of 64 pages: 1 CTA 45.5, 2 48.4, 4 55.8 (two warps); 1 CTA of four 46.9, of eight 53.0
-//   bf16, 16 x 8 items of 256 pages: 1 CTA 67.0, 2 47.6, 4 45.7, 8 49.5; 2 x 8 of 1024: 8 CTAs 37.0, of four warps 28.4
-//   fp8, 48 x 8 items of 64 pages (rings half the size, so twice the CTAs fit): 1 CTA 29.1, 2 22.6, 4 28.9
-// Short lists do not pay for the wider clusters: fp8, 16 x 8 items of 16 pages: 4 CTAs 7.1, 8 8.5; bf16, 8 x 8 of 32: 4
-// CTAs 6.4, 8 7.1; with eight heads they pay for a pair from 2048 channels on: fp8, 64 x 8 items of 8 pages 1 CTA 6.8, 2
-// 8.1; of 16 11.9, 11.2; of 48 25.8, 22.0 (sixteen heads, of 16: 18.7, 23.2: registers). Nor for a cluster at all: its
-// barriers and peers' memory cost 1.2 us, half that with an SM a CTA, and a tile costs a warp 0.35, 0.42, 0.62 us (bf16,
-// head size 64, 128, 256, up to eight heads; fp8 0.29, 0.49, 0.65), which the rule takes for 0.33, 0.44, 0.66. (Sixteen
-// heads cost 0.40, 0.52, 0.83; taken for twice the eight, since their registers let two CTAs in instead of three.) So one CTA of four warps, where the items are one wave of those
-// (registers let three in, two with sixteen heads) and the tiles a warp has more of, tiles (1/4 - 1/2c), cost less:
-//   bf16, cluster / four warps: 1 x 8 items of 4 pages 4.3 / 3.6, of 8 4.5 / 4.0, of 32 5.2 / 6.6; 16 x 8 of 8 5.8 / 4.3, of
-//   24 7.2 / 7.1, 32 x 8 of 16 8.9 / 8.2; head size 256, 1 x 8 of 8 5.3 / 5.4, 16 x 8 of 8 7.2 / 6.2
-// and instead of a CTA of two warps where each of the four has four tiles (fp8, 48 x 8 items of 16 pages 10.4 / 7.6, of 32
-// 17.1 / 13.2; head size 64, of 8 4.9 / 5.4).
+//   bf16, 64 x 8 items of 64 pages: 1 CTA 43.6, 2 46.3, 4 53.0 (two warps); 1 CTA of four 44.9
+//   bf16, 16 x 8 items of 256 pages: 1 CTA 64.4, 2 46.4, 4 43.5, 8 47.5; 2 x 8 of 1024: 8 CTAs 35.3, of four warps 27.1
+//   fp8, 48 x 8 items of 64 pages (rings half the size, so twice the CTAs fit): 1 CTA 28.2, 2 22.6, 4 28.1
+// Short lists do not pay for the wider clusters: fp8, 16 x 8 items of 16 pages: 4 CTAs 6.4, 8 8.0; bf16, 8 x 8 of 32: 4
+// CTAs 6.1, 8 7.1; with eight heads they pay for a pair from 2048 channels on: fp8, 64 x 8 items of 8 pages 1 CTA 6.6, 2
+// 8.0; of 16 11.8, 11.2; of 32 19.0, 16.3 (sixteen heads, of 16: 18.1, 22.8: registers). Nor for a cluster at all: its
+// barriers and peers' memory cost about 1 us, and a tile costs a warp 0.35, 0.42, 0.62 us (bf16, head size 64, 128, 256,
+// up to eight heads; fp8 0.29, 0.49, 0.65), which the rule takes for 0.33, 0.44, 0.66. (Sixteen heads cost 0.40, 0.52,
+// 0.83; taken for twice the eight, since their registers let two CTAs in instead of three.) So one CTA of four warps,
+// where the items are one wave of those and the tiles a warp has more of, tiles (1/4 - 1/2c), cost less:
+//   bf16, cluster / four warps: 1 x 8 items of 4 pages 4.3 / 3.4, of 8 4.3 / 3.9, of 32 5.1 / 6.3; 16 x 8 of 8 5.1 / 4.3, of
+//   32 8.5 / 8.9, 32 x 8 of 16 8.6 / 8.1; head size 256, 1 x 8 of 8 5.0 / 5.2, 16 x 8 of 8 7.0 / 6.0
+// and instead of a CTA of two warps where each of the four has four tiles (fp8, 48 x 8 items of 16 pages 10.0 / 7.5, of 32
+// 16.7 / 12.5; head size 64, of 8 5.2 / 5.5). Over 144 shapes the rule takes 1.010 of the best form's time, 1.14 at most
+// (fp8, 16 x 8 items of 64 pages 12.3, four CTAs 10.8).
 struct SparseShape { int ctas, warps; };
 static SparseShape sparse_shape(int rows, int kv_heads, int64_t tiles, int ring_bytes, int head_dim, int heads) {
   int sms = hkb_sm_count(-1);
