@@ -1,4 +1,5 @@
-// The worker of the decode over selected pages: the walk's transposed products (hkb_walk_mma.cuh) with a lazier softmax.
+// The worker of the decode over selected pages: the walk's transposed products (hkb_walk_mma.cuh) with a lazier softmax, and
+// bf16 weights in two terms.
 //
 // A warp of the dense walk is one of eight or twelve on its SM and hides its own latencies behind theirs; a selection is
 // short, its batch often small, and then one warp's chain of products, maximum, exponentials and products is what is
@@ -35,6 +36,16 @@ struct SparseWorker {
   static constexpr int STAGE_BYTES = 2 * Loader::TILE_BYTES;    // K, then V
   static constexpr int RING_SMEM = NST * STAGE_BYTES;
   static constexpr float RESCALE_LOG2 = 8.f;
+
+  // The weights meet V in 16 bits; their sum is kept of the unrounded ones. fp16's eleven bits do for fp16 answers and for
+  // an fp8 cache's bf16 ones (error against float64 0.00027 of the norm, rounded once 0.00021; 0.0017, 0.0017). bf16's eight
+  // do not (0.0023, 0.0017), so a bf16 weight is two terms, its upper half and what is left, multiplied one after the other
+  // by the V fragment that is there: 0.0017. Both are positive, or an infinite value would meet 0 or two signs and be NaN.
+  static constexpr int TERMS = KIND == HKB_KV_BF16 ? 2 : 1;
+  __device__ static __forceinline__ uint32_t upper16x2(float lo, float hi) {
+    return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+  }
+  __device__ static __forceinline__ float rest(float x) { return fmaxf(x - bf16hi(__float_as_uint(x)), 0x1p-126f); }
 
   // As the walk's, but for an fp8 cache's query, which the walk cuts at f16's range: here each head is scaled into it, and
   // NaN and infinities stay what they are.
@@ -146,7 +157,7 @@ struct SparseWorker {
           st.m[nt][c] = mx;
         }
     }
-    uint32_t pb[NT][2];
+    uint32_t pb[NT][2], pr[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float mu0 = st.m[nt][0] == -INFINITY ? 0.f : -st.m[nt][0], mu1 = st.m[nt][1] == -INFINITY ? 0.f : -st.m[nt][1];
@@ -155,11 +166,15 @@ struct SparseWorker {
       const float p2 = fast_exp2(fmaf(sc[nt][2], qs0, mu0)), p3 = fast_exp2(fmaf(sc[nt][3], qs1, mu1));
       st.l[nt][0] += p0 + p2;
       st.l[nt][1] += p1 + p3;
-      // The weights meet V in 16 bits, as in the dense walk; their sum is kept of the unrounded ones. A bf16 answer is off
-      // by 0.0023 of its norm so, 0.0017 where it is rounded once. Two bf16 terms a weight reach that for 1 % of the time
-      // (45.4 to 45.9 us for 64 x 8 items of 64 pages), but make NaN of an infinite value, which meets terms of both signs.
-      pb[nt][0] = movmatrix_trans(pack16x2<F16>(p0, p1));
-      pb[nt][1] = movmatrix_trans(pack16x2<F16>(p2, p3));
+      if constexpr (TERMS == 1) {
+        pb[nt][0] = movmatrix_trans(pack16x2<F16>(p0, p1));
+        pb[nt][1] = movmatrix_trans(pack16x2<F16>(p2, p3));
+      } else {
+        pb[nt][0] = movmatrix_trans(upper16x2(p0, p1));
+        pb[nt][1] = movmatrix_trans(upper16x2(p2, p3));
+        pr[nt][0] = movmatrix_trans(pack_bf16x2(rest(p0), rest(p1)));
+        pr[nt][1] = movmatrix_trans(pack_bf16x2(rest(p2), rest(p3)));
+      }
     }
     if constexpr (FP8) {
 #pragma unroll
@@ -183,7 +198,10 @@ struct SparseWorker {
         uint32_t a[4];
         ldmatrix_x4_trans(a, vtile + tile_off<D * 2>(r, dt * 2 + ((lane >> 3) & 1)));
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16<F16>(st.o[nt][dt], a, pb[nt]);
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16<F16>(st.o[nt][dt], a, pb[nt]);
+          if constexpr (TERMS == 2) mma16<F16>(st.o[nt][dt], a, pr[nt]);
+        }
       }
     }
   }

@@ -154,16 +154,17 @@ def select_ref(scores, lens, page, budget, first, last):
 
 # ------------------------------------------------------------------------- attention
 
-def sparse_ref(q, key_cache, value_cache, table, lens, pages, scale, k_scale=None, v_scale=None):
+def sparse_ref(q, key_cache, value_cache, table, lens, pages, scale, k_scale=None, v_scale=None, terms=1):
     """(out, out tolerance, lse, lse tolerance), float64. What the kernel rounds: q.k is exact products added in fp32
     (2^-23 of the sum of magnitudes an addition), the exponential's argument and the exponential (2^-21 together), the
     weights to 16 bits before they meet V -- the activation type's u, fp16's for an fp8 cache, plus fp16's smallest
-    step under values of 1 and more -- and the answer to the activation type."""
+    step under values of 1 and more -- and the answer to the activation type. `terms` 2: a weight is its upper half and,
+    below 2^-7 of it, the rest rounded to bf16."""
     rows, hq, d = q.shape
     page, hkv = key_cache.shape[1], key_cache.shape[2]
     g = hq // hkv
     fp8 = key_cache.dtype not in U16
-    up = 2.0 ** -11 if fp8 else U16[q.dtype]
+    up = 2.0 ** -11 if fp8 else U16[q.dtype] if terms == 1 else 2.0 ** -7 * U16[torch.bfloat16]
     out = torch.zeros(rows, hq, d, dtype=torch.float64)
     tol = torch.zeros_like(out)
     lse = torch.full((rows, hq), -math.inf, dtype=torch.float64)

@@ -271,3 +271,33 @@ def test_several_tokens_of_one_sequence(kv):
     part = dict(c, table=table[:1].cuda().expand(4, -1), lens=lens[:4], q=c["q"][:4])      # a row stride of 0
     got, _ = _attend(part, pages[:4].cpu())
     assert torch.equal(got, out[:4])
+
+
+# ------------------------------------------------------------------------------ weights
+
+@pytest.mark.parametrize("d, group, budget", [(64, 4, 12), (128, 8, 30), (256, 12, 7)])
+def test_bf16_weights_are_not_rounded_to_bf16(d, group, budget):
+    """Logits of nearly nothing, so that the weights' own rounding would be seen: they are held to 2^-15, not bf16's 2^-8."""
+    c = _cache_case([200, 37, 480], d=d, h_kv=2, group=group, seed=d + 1)
+    c["scale"] = 2.0 ** -12
+    pages = _random_pages(c, budget)
+    got, lse = _attend(c, pages)
+    want, tol, wl, tl = orc.sparse_ref(c["q"], c["k"], c["v"], c["table"], c["lens"], pages, c["scale"], terms=2)
+    _hold(got, want, tol)
+    _hold(lse, wl, tl)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "f16"])
+def test_an_infinite_value_makes_its_channel_infinite(kv):
+    """Its weight is positive; no other channel, head or row changes, and behind a sequence's end it is not met."""
+    c = _cache_case([300, 90, 37], d=128, h_kv=2, group=4, kv=kv, seed=19)
+    pages = _random_pages(c, 20)
+    want, lse = _attend(c, pages)
+    c["v"][int(c["table"][0, 3]), 5, 1, 77] = math.inf
+    c["v"][int(c["table"][1, 5]), 9, 0, 3] = -math.inf
+    c["v"][int(c["table"][2, 2]), 5, 0, 9] = math.inf         # position 37 of 37 tokens
+    got, lse2 = _attend(c, pages)
+    hit = torch.zeros(want.shape, dtype=torch.bool)
+    hit[0, 4:, 77] = hit[1, :4, 3] = True
+    assert torch.isposinf(got[0, 4:, 77]).all() and torch.isneginf(got[1, :4, 3]).all()
+    assert torch.equal(got[~hit.cuda()], want[~hit.cuda()]) and torch.equal(lse2, lse)
