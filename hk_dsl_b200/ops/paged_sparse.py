@@ -178,7 +178,9 @@ def update_page_bounds(bounds: torch.Tensor, key_cache: torch.Tensor, block_tabl
     below `num_tokens`, the step's rows (a host number): the starts run on past it where `advance_tables` refused a
     request for rows. A sequence without new tokens has its last page summarised again: it holds fewer tokens if the
     sequence was shortened. `bounds` is of the cache's type: nothing is rounded. Pages
-    are read from the cache as it is, so a call may be repeated; sequences of length 0 are left out."""
+    are read from the cache as it is, so a call may be repeated; sequences of length 0 are left out. The table has one row a
+    sequence (not one a query row, where those are several a sequence): a page that two rows share must be full in both, or
+    which of them its summary is of depends on the order."""
     (nb, page, hkv, d), ks, _ = _cache_strides(key_cache)
     bshape, bs = _bounds_strides(bounds)
     code = _kind(key_cache)

@@ -508,7 +508,8 @@ int hkb_advance_tables(const hkb_advance_t* args, void* stream);
  * of q_start past it counts as it. A sequence without new tokens has its last page summarised again, which holds fewer
  * tokens if the sequence was shortened. bounds has the cache's element type (values are kept exactly, fp8 ones as
  * stored); its last two axes are contiguous, head_dim each. A NaN key makes the channel's bounds NaN. Page ids outside
- * [0, min(bounds_blocks, k_cache.num_blocks)) are skipped. block_size is any positive number.
+ * [0, min(bounds_blocks, k_cache.num_blocks)) are skipped. A page that two sequences share must be full in both.
+ * block_size is any positive number.
  */
 typedef struct {
   void* bounds;
