@@ -480,8 +480,8 @@ __global__ void __launch_bounds__(BOUNDS_WARPS * 32) bounds_kernel(const BoundsA
 // lane then reads nothing that another one fetched, the copies run through a cp.async ring in which every lane has its
 // own 16-byte places: asynchronous and deep as a walk's ring, without a barrier or a swizzle.
 // Bound: bytes (a summary is 2 rows a page where the attention reads 2 rows a token). Measured: 2 x 8192 pages, eight kv
-// heads of eight query heads, 13.1 us = 5.2 TB/s (loads straight into registers, two tiles a warp: 14.7 to 16; rings in
-// CTAs of four warps instead of one: 17.0, one chain of products a score: 17.3); four sequences of up to 32 pages 1.9 us.
+// heads of eight query heads, 13.2 us = 5.1 TB/s (loads straight into registers, two tiles a warp: 14.7 to 16; rings in
+// CTAs of four warps instead of one: 17.0, one chain of products a score: 17.3); four sequences of up to 32 pages 2.0 us.
 // ---------------------------------------------------------------------------------
 constexpr int SCORE_WARPS = 1;
 template <int D, bool FP8>

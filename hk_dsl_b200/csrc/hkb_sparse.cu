@@ -196,21 +196,21 @@ __global__ void __launch_bounds__(WARPS * 32, sparse_ctas<P, WARPS>()) sparse_ke
 // portable cluster: more only adds waves of them (each costs about 6 us whatever it does), fewer leave a batch of few
 // rows to few warps. Where even eight CTAs of two warps leave half the machine's mma pipes idle and each warp has more
 // than eight tiles to go, four warps a CTA. Measured at head size 128, 16-token pages, us:
-//   bf16, 64 x 8 items of 64 pages: 1 CTA 43.6, 2 46.3, 4 53.0 (two warps); 1 CTA of four 44.9
-//   bf16, 16 x 8 items of 256 pages: 1 CTA 64.4, 2 46.4, 4 43.5, 8 47.5; 2 x 8 of 1024: 8 CTAs 35.3, of four warps 27.1
-//   fp8, 48 x 8 items of 64 pages (rings half the size, so twice the CTAs fit): 1 CTA 28.2, 2 22.6, 4 28.1
+//   bf16, 64 x 8 items of 64 pages: 1 CTA 43.8, 2 46.6, 4 53.4 (two warps); 1 CTA of four 45.3
+//   bf16, 16 x 8 items of 256 pages: 1 CTA 69.3, 2 47.3, 4 44.0, 8 47.8; 2 x 8 of 1024: 8 CTAs 37.3, of four warps 27.5
+//   fp8, 48 x 8 items of 64 pages (rings half the size, so twice the CTAs fit): 1 CTA 28.2, 2 22.6, 4 27.6
 // Short lists do not pay for the wider clusters: fp8, 16 x 8 items of 16 pages: 4 CTAs 6.4, 8 8.0; bf16, 8 x 8 of 32: 4
-// CTAs 6.1, 8 7.1; with eight heads they pay for a pair from 2048 channels on: fp8, 64 x 8 items of 8 pages 1 CTA 6.6, 2
-// 8.0; of 16 11.8, 11.2; of 32 19.0, 16.3 (sixteen heads, of 16: 18.1, 22.8: registers). Nor for a cluster at all: its
-// barriers and peers' memory cost about 1 us, and a tile costs a warp 0.35, 0.42, 0.62 us (bf16, head size 64, 128, 256,
-// up to eight heads; fp8 0.29, 0.49, 0.65), which the rule takes for 0.33, 0.44, 0.66. (Sixteen heads cost 0.40, 0.52,
-// 0.83; taken for twice the eight, since their registers let two CTAs in instead of three.) So one CTA of four warps,
+// CTAs 6.3, 8 7.1; with eight heads they pay for a pair from 2048 channels on: fp8, 64 x 8 items of 8 pages 1 CTA 6.6, 2
+// 8.0; of 16 11.7, 11.3; of 32 18.7, 16.3 (sixteen heads, of 16: 18.1, 22.8: registers). Nor for a cluster at all: its
+// barriers and peers' memory cost about 1 us, and a tile costs a warp 0.37, 0.48, 0.70 us (bf16, head size 64, 128, 256,
+// up to eight heads; fp8 0.30, 0.49, 0.65), which the rule takes for 0.33, 0.44, 0.66. (Sixteen heads cost 0.46, 0.60,
+// 1.00; taken for twice the eight, since their registers let two CTAs in instead of three.) So one CTA of four warps,
 // where the items are one wave of those and the tiles a warp has more of, tiles (1/4 - 1/2c), cost less:
-//   bf16, cluster / four warps: 1 x 8 items of 4 pages 4.3 / 3.4, of 8 4.3 / 3.9, of 32 5.1 / 6.3; 16 x 8 of 8 5.1 / 4.3, of
-//   32 8.5 / 8.9, 32 x 8 of 16 8.6 / 8.1; head size 256, 1 x 8 of 8 5.0 / 5.2, 16 x 8 of 8 7.0 / 6.0
+//   bf16, cluster / four warps: 1 x 8 items of 4 pages 4.3 / 3.5, of 8 4.4 / 4.0, of 32 5.2 / 6.7; 16 x 8 of 8 5.2 / 4.4, of
+//   32 8.8 / 9.2, 32 x 8 of 16 8.9 / 8.3; head size 256, 1 x 8 of 8 5.1 / 5.4, 16 x 8 of 8 7.1 / 6.1
 // and instead of a CTA of two warps where each of the four has four tiles (fp8, 48 x 8 items of 16 pages 10.0 / 7.5, of 32
-// 16.7 / 12.5; head size 64, of 8 5.2 / 5.5). Over 144 shapes the rule takes 1.010 of the best form's time, 1.14 at most
-// (fp8, 16 x 8 items of 64 pages 12.3, four CTAs 10.8).
+// 16.7 / 12.5; head size 64, of 8 5.2 / 5.5). Over 144 shapes the rule takes 1.009 of the best form's time, 1.15 at most
+// (fp8, 16 x 8 items of 64 pages 12.4, four CTAs 10.8).
 struct SparseShape { int ctas, warps; };
 static SparseShape sparse_shape(int rows, int kv_heads, int64_t tiles, int ring_bytes, int head_dim, int heads) {
   int sms = hkb_sm_count(-1);

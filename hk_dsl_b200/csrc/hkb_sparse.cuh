@@ -6,9 +6,10 @@
 // waited for. So a score is added up in two chains of products (the fp8 walk does that too), and where the dense walks
 // exchange every tile's maximum to compare it with the softmax reference, here a lane compares its own scores, and only
 // if one of the warp's exceeds the reference by 2^8 (the first tile, and rarely after) are maxima exchanged and the
-// accumulators rescaled: 16 x 8 items of 256 pages, a CTA of two warps each, 67 us instead of 77. A tile (bf16, head size
-// 128) then costs a warp 0.42 us where its SM holds no other CTA and 0.47 where all SMs are full; what is left is the
-// issue of its instructions one after another (the tensor pipe is 16 % busy at twelve warps an SM). Two tiles a step took 0.48 us each and twice the shared memory: 16 x 8 items of 256
+// accumulators rescaled: 16 x 8 items of 256 pages, a CTA of two warps each and one bf16 term a weight, 67 us instead of
+// 77. A tile (bf16, head size 128, two terms) costs a warp 0.48 us where its SM holds no other CTA and 0.51 where all SMs
+// are full (0.42 and 0.47 with one); what is left is the issue of its instructions one after another (the tensor pipe is
+// 16 % busy at twelve warps an SM). Two tiles a step took 0.48 us each and twice the shared memory: 16 x 8 items of 256
 // pages 61 against 67 us on a CTA each, but 64 x 8 of 64 pages 48.3 against 45.4, where the rings are what is short.
 #pragma once
 
