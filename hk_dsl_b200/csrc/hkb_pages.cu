@@ -540,6 +540,21 @@ __device__ __forceinline__ float score_by_definition(const __nv_bfloat16* q, int
   return best;
 }
 
+// Whether a NaN is among a group's 16-bit query heads.
+template <int KIND, int D>
+__device__ __forceinline__ int query_is_broken(const __nv_bfloat16* q, int64_t q_stride_head, int group, int lane) {
+  constexpr uint32_t INF = KIND == HKB_KV_F16 ? 0x7c00u : 0x7f80u;
+  bool nan = false;
+#pragma unroll 1
+  for (int x = lane; x < group * (D / 8); x += 32) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(q + (int64_t)(x / (D / 8)) * q_stride_head + x % (D / 8) * 8));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) nan |= (w[i] & 0x7fffu) > INF || (w[i] >> 16 & 0x7fffu) > INF;
+  }
+  return __any_sync(0xffffffffu, nan);
+}
+
 template <int KIND, int D, int NT>
 __global__ void __launch_bounds__(SCORE_WARPS * 32, 8) scores_kernel(const ScoreArgs a) {
   constexpr bool FP8 = KIND == HKB_KV_FP8_E4M3, F16 = KIND != HKB_KV_BF16;   // e4m3 widens to f16 exactly
@@ -626,6 +641,7 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32, 8) scores_kernel(const Score
   const float factor = a.scale * (a.k_scale ? __ldg(a.k_scale) : 1.f);
 
   int stage = 0, stage_next = Ring::STAGES - 1;
+  int broken = -1;                             // whether the query has a NaN: not known
   for (int p0 = first; p0 < end; p0 += 16) {
     cp_async_wait<Ring::STAGES - 2>();         // this lane's own copies: nobody else's are read
     const uint32_t tile = ring + stage * Ring::TILE;
@@ -692,8 +708,13 @@ __global__ void __launch_bounds__(SCORE_WARPS * 32, 8) scores_kernel(const Score
     float mine = t & 1 ? best[1] : best[0];
     if constexpr (!FP8) {
       // The rewritten product meets the half of the wrong sign with a zero, and of an infinite bound that is NaN though
-      // max(q low, q high) may be finite: pages without a number are computed again. (e4m3 has no infinities.)
-      for (unsigned bad = __ballot_sync(0xffffffffu, t < 2 && p < end && mine != mine); bad; bad &= bad - 1) {
+      // max(q low, q high) may be finite: pages without a number are computed again. (e4m3 has no infinities.) Not if the
+      // query has none itself, or its row would cost a batch some hundred microseconds.
+      unsigned bad = __ballot_sync(0xffffffffu, t < 2 && p < end && mine != mine);
+      if (bad && broken < 0)
+        broken = query_is_broken<KIND, D>(a.q + (int64_t)row * a.q_stride_row + (int64_t)(head * a.group) * a.q_stride_head, a.q_stride_head, a.group, lane);
+      if (broken > 0) bad = 0;
+      for (; bad; bad &= bad - 1) {
         const int from = __ffs(bad) - 1;
         const int id = __ldg(table + __shfl_sync(0xffffffffu, p, from));
         const uint8_t* low = a.bounds + (int64_t)min(max(id, 0), a.num_blocks - 1) * a.b_stride_block + (int64_t)head * a.b_stride_head;

@@ -162,6 +162,22 @@ def test_page_scores_of_infinite_bounds_are_the_definitions(kv, d, group):
     _hold(got, want, tol)
 
 
+@pytest.mark.parametrize("kv", ["bf16", "f16", "fp8"])
+@pytest.mark.parametrize("d, group", [(64, 4), (128, 12), (256, 16)])
+def test_page_scores_of_a_broken_query(kv, d, group):
+    """A NaN in any head of a group makes all pages of its row and kv head NaN, and no others."""
+    c = _cache_case([16 * 30, 16 * 7 + 1, 400], d=d, h_kv=2, group=group, kv=kv, seed=d + group)
+    b = _bounds_of(c)
+    for r, h, x in ((0, 0, d - 1), (1, 2 * group - 1, 0), (2, group - 1, d // 2 + 1)):
+        c["q"][r, h, x] = -math.nan if r else math.nan
+    want, tol = orc.scores_ref(c["q"], b, c["table"], c["lens"], 16, c["scale"], c["ks"])
+    assert torch.isnan(want[0, 0, :30]).all() and torch.isnan(want[1, 1, :8]).all() and torch.isfinite(want[0, 1, :30]).all()
+    got = torch.full(want.shape, 5.0, device="cuda")
+    _ps().page_scores(got, c["q"].cuda(), b.cuda(), c["table"].cuda(), _lens(c), c["scale"], 16, c["name"], _cu(c["ks"]))
+    assert torch.equal(torch.isnan(got.cpu()), torch.isnan(want))
+    _hold(got, want, tol)
+
+
 # ------------------------------------------------------------------------------ the integers' ends
 
 def test_advance_tables_takes_back_as_many_pages_as_an_int_counts():
