@@ -102,7 +102,9 @@ def advance_tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, new_token
     `slot_mapping` and `positions` (rows,) int64 of every new token in that order, -1 and 0 in the rows behind the last
     one (`reshape_and_cache` skips them, so a captured step may have spare rows); `status` (requests,) int32. A request
     with `REQ_NO_PAGES` (too few free pages; once one is short, so is every later one that needs any), `REQ_TABLE_FULL`
-    or `REQ_NO_ROWS` keeps its length, gets no page, and its rows get slot -1. A page belongs to one request."""
+    or `REQ_NO_ROWS` keeps its length, gets no page, and its rows get slot -1. The tokens it asked for are counted in
+    `query_start_loc` all the same: behind a `REQ_NO_ROWS` the starts lie past `rows`, and a call that reads query rows by them
+    must not be made before `status` was looked at. A page belongs to one request."""
     _index("block_tables", block_tables, 2)
     for t in (seq_lens, new_tokens, free_pages, free_count, query_start_loc, status):
         if t.dtype is not _I32 or t.stride() != (1,):

@@ -465,6 +465,8 @@ int hkb_paged_decode_static(void* out, int64_t out_stride_tok, int64_t out_strid
  * more; a negative value gives that many back from its end (rejected drafts; a whole length: a finished
  * request). Free pages are the stack free_pages[0 .. *free_count).
  *   - q_start[i], num_reqs + 1 entries: where the request's new tokens begin among the step's rows, in request order.
+ *     Refused requests are counted too, so behind an HKB_REQ_NO_ROWS the entries lie past num_rows: whoever reads query
+ *     rows by them looks at status first. (hkb_page_bounds takes them as they are.)
  *   - slot_mapping[t], positions[t] (int64, num_rows entries): row t's slot page * block_size + offset and its
  *     position. Rows behind the last request's: slot -1, position 0. (hkb_reshape_and_cache skips slot -1.)
  *   - status[i]: HKB_REQ_*. A refused request keeps its length and gets no page; its rows get slot -1.
